@@ -8,6 +8,7 @@ LIB_PATH = os.environ.get("CARD_AMD_LIB") or os.path.join(_HERE, "libcard_hip.so
 CARD_OK = 0
 VARIANT_GUIDED, VARIANT_BN_HADAMARD, VARIANT_LINEAR_HADAMARD = 0, 1, 2
 OUT_LAST, OUT_ALL, OUT_SELECT = 0, 1, 2
+DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_E4M3 = 0, 1, 2, 3
 ARITH_F32_MFMA, ARITH_SPLIT_BF16 = 0, 1
 COEF_COLS = 8
 
@@ -16,8 +17,13 @@ EXPORTS = (
     "card_sampler_run", "card_sampler_workspace_bytes", "card_eps_theta", "card_q_sample", "card_philox_normal",
     "card_regression_row_metrics", "card_classification_row_metrics", "card_sampler_run_static", "card_content_hash",
     "card_fphi_create", "card_fphi_destroy", "card_fphi_forward", "card_sampler_plan",
+    "card_dropout", "card_dropout_backward", "card_rms_norm", "card_rms_norm_backward",
+    "card_rms_norm_backward_workspace_bytes", "card_linear4_create", "card_linear4_destroy", "card_linear4_forward",
+    "card_linear4_quantize",
 )
 FPHI_MAX_LAYERS, FPHI_MAX_WIDTH = 8, 1024
+NORM_MAX_COLS = 65536
+LINEAR4_MAX_FEATURES, LINEAR4_MAX_ROWS = 1048576, 65535
 STATIC_SCRATCH_BYTES = 32 << 20
 
 _fp = C.c_void_p  # device pointers travel as integers (tensor.data_ptr())
@@ -76,6 +82,13 @@ class ClsMetricArgs(C.Structure):
     ]
 
 
+class Linear4Desc(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_int32), ("in_features", C.c_int32), ("out_features", C.c_int32), ("group", C.c_int32),
+        ("q", _fp), ("scale", _fp), ("zero", _fp), ("bias", _fp),
+    ]
+
+
 class CardError(RuntimeError):
     pass
 
@@ -114,6 +127,17 @@ def lib():
     L.card_fphi_destroy.restype = None
     L.card_fphi_forward.argtypes = [C.c_void_p, _fp, C.c_int64, _fp, C.c_void_p]
     L.card_philox_normal.argtypes = [C.c_uint64, C.c_uint64, C.c_int64, C.c_int32, C.c_int32, _fp, C.c_void_p]
+    i32, i64, u64, f64 = C.c_int32, C.c_int64, C.c_uint64, C.c_double
+    L.card_dropout.argtypes = [_fp, _fp, _fp, i32, i64, i64, i32, f64, u64, u64, _fp, i32, C.c_void_p]
+    L.card_dropout_backward.argtypes = [_fp, _fp, i32, i64, i64, i32, f64, u64, u64, _fp, i32, C.c_void_p]
+    L.card_rms_norm.argtypes = [_fp, _fp, _fp, i32, i32, i64, i64, f64, _fp, _fp, i32, _fp, C.c_void_p]
+    L.card_rms_norm_backward_workspace_bytes.argtypes = [i32, i64, i64, C.POINTER(u64)]
+    L.card_rms_norm_backward.argtypes = [_fp, _fp, _fp, _fp, i32, i32, i64, i64, f64, _fp, _fp, _fp, u64, C.c_void_p]
+    L.card_linear4_create.argtypes = [C.POINTER(Linear4Desc), C.c_void_p, C.POINTER(C.c_void_p)]
+    L.card_linear4_destroy.argtypes = [C.c_void_p]
+    L.card_linear4_destroy.restype = None
+    L.card_linear4_forward.argtypes = [C.c_void_p, _fp, i32, _fp, i64, _fp, C.c_float, _fp, i32, C.c_void_p]
+    L.card_linear4_quantize.argtypes = [_fp, i32, i32, i32, _fp, _fp, _fp, C.c_void_p]
     for name in EXPORTS:
         getattr(L, name)  # AttributeError here = a symbol the header declares is not exported
     _lib = L

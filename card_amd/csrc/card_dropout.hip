@@ -1,0 +1,156 @@
+// card_dropout.hip - dropout whose mask is a function of (seed, element, draw) and is never stored.
+//
+//   y[r, z, c] = residual[r, z, c] + keep(e) * x[r, c] / (1 - p),   e = elem_offset + ((r * n_z + z) * cols + c)
+//   dx[r, c]   = sum over z of keep(e) * g[r, z, c] / (1 - p)       (the residual's gradient is g itself)
+//
+// Backward makes the same mask again from the same numbers: nothing of the forward pass is kept but the seed.
+#include "card_layers.h"
+
+using namespace card;
+
+int drop_rule(const char* who, double p, uint64_t seed, uint64_t elem_offset, const uint64_t* state, int32_t draw, DropRule* d) {
+    if (!(p >= 0.0 && p <= 1.0)) return card_fail(CARD_E_INVALID, "%s: p=%g outside [0, 1]", who, p);
+    if (draw < 0) return card_fail(CARD_E_INVALID, "%s: draw=%d < 0", who, draw);
+    if (elem_offset >> 63) return card_fail(CARD_E_INVALID, "%s: elem_offset beyond 2^63", who);
+    const double t = nearbyint(p * 4294967296.0);
+    d->seed = seed; d->elem_offset = elem_offset; d->state = (const unsigned long long*)state; d->draw = (uint32_t)draw;
+    d->none = t >= 4294967296.0;
+    d->threshold = d->none ? 0xFFFFFFFFu : (uint32_t)t;
+    d->scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.0f;
+    return CARD_OK;
+}
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct Shape {
+    long long cols;        // elements of a row of the output
+    long long per_row;     // chunks of a row
+    long long chunks;      // rows * n_z * per_row
+    int n_z;
+};
+
+// One thread per chunk of 16 bytes of the output.  n_z = 1 is one long row, so that only the tensor's end is ragged.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void dropout_kernel(const Shape s, const DropRule d, const T* x, const T* residual, T* out) {
+    constexpr int N = 16 / sizeof(T);
+    const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
+    if (id >= s.chunks) return;
+    unsigned long long seed, off;
+    drop_key(d, seed, off);
+    const long long rz = s.per_row == s.chunks ? 0 : id / s.per_row, c = (id - rz * s.per_row) * N;
+    const long long n = s.cols - c, at = rz * s.cols + c, from = (s.n_z == 1 ? rz : rz / s.n_z) * s.cols + c;
+    float v[N], r[N];
+    load_n<N>(x + from, n, v);
+    if (residual) load_n<N>(residual + at, n, r);
+    const uint32_t m = keep_bits<N>(d, seed, off + (unsigned long long)at, n < N ? (int)n : N);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i] = (m >> i) & 1 ? v[i] * d.scale : 0.0f;
+        if (residual) v[i] += r[i];
+    }
+    store_n<N>(out + at, n, v);
+}
+
+// n_z > 1: lanes_z threads of a workgroup share one chunk of x, each takes every lanes_z-th mask, and their sums are joined
+// in a fixed order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void dropout_backward_kernel(const Shape s, const DropRule d, const T* g, T* dx, int lanes_z) {
+    constexpr int N = 16 / sizeof(T);
+    __shared__ float part[kThreads][N + 1];
+    const int per_wg = kThreads / lanes_z, sub = threadIdx.x / per_wg;
+    const long long id = (long long)blockIdx.x * per_wg + threadIdx.x % per_wg;      // chunk of x
+    const bool live = id < s.chunks / s.n_z;
+    unsigned long long seed, off;
+    drop_key(d, seed, off);
+    float sum[N] = {};
+    const long long row = live ? id / s.per_row : 0, c = live ? (id - row * s.per_row) * N : 0, n = s.cols - c;
+    if (live) {
+        for (int z = sub; z < s.n_z; z += lanes_z) {
+            const long long at = (row * s.n_z + z) * s.cols + c;
+            float v[N];
+            load_n<N>(g + at, n, v);
+            const uint32_t m = keep_bits<N>(d, seed, off + (unsigned long long)at, n < N ? (int)n : N);
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += (m >> i) & 1 ? v[i] : 0.0f;
+        }
+    }
+    if (lanes_z > 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) part[threadIdx.x][i] = sum[i];
+        __syncthreads();
+        if (sub == 0)
+            for (int k = 1; k < lanes_z; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] += part[threadIdx.x + k * per_wg][i];
+    }
+    if (!live || sub) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] *= d.scale;
+    store_n<N>(dx + row * s.cols + c, n, sum);
+}
+
+int shape_of(const char* who, int32_t dtype, int64_t rows, int64_t cols, int32_t n_z, Shape* s) {
+    const int64_t eb = card_dtype_bytes(dtype);
+    if (dtype == CARD_DTYPE_E4M3 || !eb) return card_fail(CARD_E_INVALID, "%s: dtype %d is none of CARD_DTYPE_F32, _BF16, _F16", who, dtype);
+    if (rows < 0 || cols < 0) return card_fail(CARD_E_INVALID, "%s: rows=%lld or cols=%lld < 0", who, (long long)rows, (long long)cols);
+    if (n_z < 1) return card_fail(CARD_E_INVALID, "%s: n_z=%d < 1", who, n_z);
+    int64_t all;
+    if (__builtin_mul_overflow(rows, cols, &all) || __builtin_mul_overflow(all, (int64_t)n_z * eb, &all))
+        return card_fail(CARD_E_INVALID, "%s: more bytes than 63 bits count", who);
+    const int64_t n = 16 / eb;
+    if (n_z == 1) { cols *= rows; rows = 1; }
+    s->cols = cols; s->n_z = n_z; s->per_row = (cols + n - 1) / n; s->chunks = rows * n_z * s->per_row;
+    if (s->chunks > (int64_t)kThreads * 0x7fffffff) return card_fail(CARD_E_UNSUPPORTED, "%s: more than 2^31 workgroups", who);
+    return CARD_OK;
+}
+
+template <typename T> int forward(const Shape& s, const DropRule& d, const void* x, const void* residual, void* out, hipStream_t stream) {
+    const unsigned grid = (unsigned)((s.chunks + kThreads - 1) / kThreads);
+    dropout_kernel<T><<<grid, kThreads, 0, stream>>>(s, d, (const T*)x, (const T*)residual, (T*)out);
+    HIP_TRY(hipGetLastError());
+    return CARD_OK;
+}
+
+template <typename T> int backward(const Shape& s, const DropRule& d, const void* g, void* dx, hipStream_t stream) {
+    if (s.n_z == 1) return forward<T>(s, d, g, nullptr, dx, stream);
+    const long long chunks = s.chunks / s.n_z;
+    int lanes = 1;
+    while (lanes < 64 && 2 * lanes <= s.n_z && chunks * lanes < 1 << 18) lanes *= 2;
+    const long long per_wg = kThreads / lanes, grid = (chunks + per_wg - 1) / per_wg;
+    if (grid > 0x7fffffff) return card_fail(CARD_E_UNSUPPORTED, "card_dropout_backward: more than 2^31 workgroups");
+    dropout_backward_kernel<T><<<(unsigned)grid, kThreads, 0, stream>>>(s, d, (const T*)g, (T*)dx, lanes);
+    HIP_TRY(hipGetLastError());
+    return CARD_OK;
+}
+
+}  // namespace
+
+extern "C" CARD_API int card_dropout(const void* x, const void* residual, void* out, int32_t dtype, int64_t rows, int64_t cols,
+                                     int32_t n_z, double p, uint64_t seed, uint64_t elem_offset, const uint64_t* state,
+                                     int32_t draw, void* stream) {
+    Shape s;
+    DropRule d;
+    int rc = shape_of("card_dropout", dtype, rows, cols, n_z, &s);
+    if (rc == CARD_OK) rc = drop_rule("card_dropout", p, seed, elem_offset, state, draw, &d);
+    if (rc != CARD_OK || s.chunks == 0) return rc;
+    if (!x || !out) return card_fail(CARD_E_INVALID, "card_dropout: null x / out");
+    hipStream_t st = (hipStream_t)stream;
+    return dtype == CARD_DTYPE_F32 ? forward<float>(s, d, x, residual, out, st)
+         : dtype == CARD_DTYPE_BF16 ? forward<bf16_t>(s, d, x, residual, out, st) : forward<f16_t>(s, d, x, residual, out, st);
+}
+
+extern "C" CARD_API int card_dropout_backward(const void* g, void* dx, int32_t dtype, int64_t rows, int64_t cols, int32_t n_z,
+                                              double p, uint64_t seed, uint64_t elem_offset, const uint64_t* state, int32_t draw,
+                                              void* stream) {
+    Shape s;
+    DropRule d;
+    int rc = shape_of("card_dropout_backward", dtype, rows, cols, n_z, &s);
+    if (rc == CARD_OK) rc = drop_rule("card_dropout_backward", p, seed, elem_offset, state, draw, &d);
+    if (rc != CARD_OK || s.chunks == 0) return rc;
+    if (!g || !dx) return card_fail(CARD_E_INVALID, "card_dropout_backward: null g / dx");
+    hipStream_t st = (hipStream_t)stream;
+    return dtype == CARD_DTYPE_F32 ? backward<float>(s, d, g, dx, st)
+         : dtype == CARD_DTYPE_BF16 ? backward<bf16_t>(s, d, g, dx, st) : backward<f16_t>(s, d, g, dx, st);
+}

@@ -325,6 +325,78 @@ typedef struct card_cls_metric_args {
 
 CARD_API int card_classification_row_metrics(const card_cls_metric_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Layer operators: what surrounds a Linear in a guidance network or a conditional head -- dropout, root-mean-square norm,
+ * products of few rows with 4-bit weights.  NO COUNTERPART IN THE REFERENCE'S NATIVE CODE (it has none); its f_phi holds
+ * nn.Dropout after every hidden layer (regression/model.py:77).  As everywhere: device pointers, row-major, contiguous, any
+ * alignment that suits the element, stream-ordered, no synchronisation; outputs overlap no input.
+ * ------------------------------------------------------------------------------------------------------------------ */
+typedef enum card_dtype {
+    CARD_DTYPE_F32 = 0,
+    CARD_DTYPE_BF16 = 1,
+    CARD_DTYPE_F16 = 2,
+    CARD_DTYPE_E4M3 = 3 /* 8 bits: 4 of exponent, 3 of mantissa, no infinities, largest value 448 */
+} card_dtype;
+
+/* out[r, z, c] = residual[r, z, c] + keep(e) * x[r, c] / (1 - p) with e = elem_offset + ((r * n_z + z) * cols + c).
+ * x (rows, cols); residual (rows, n_z, cols) or NULL; out (rows, n_z, cols): n_z masks of every row, as the sampler's n_z.
+ * keep(e): word e & 3 of Philox4x32-10 at counter (low and high word of e >> 2, draw, 1) under the key `seed` is at least
+ * round(p * 2^32).  (The sampler's normals use 0 as the last counter word: one seed serves both.)  A dropped element is 0
+ * whatever x holds there; p = 1 drops everything.  state: NULL, or two device words {seed, element offset} that are read
+ * when the kernel runs: the seed replaces `seed`, the offset is added to elem_offset (a captured graph then draws a new mask
+ * whenever the words change).  dtype: CARD_DTYPE_F32, _BF16, _F16; sums are fp32, rounded once.  0 <= p <= 1, draw >= 0,
+ * elem_offset < 2^63. */
+CARD_API int card_dropout(const void* x, const void* residual, void* out, int32_t dtype, int64_t rows, int64_t cols, int32_t n_z,
+                          double p, uint64_t seed, uint64_t elem_offset, const uint64_t* state, int32_t draw, void* stream);
+/* dx[r, c] = sum over z of keep(e) * g[r, z, c] / (1 - p), with the mask of the same arguments (the residual's gradient is g).
+ * The sum over z has a fixed order. */
+CARD_API int card_dropout_backward(const void* g, void* dx, int32_t dtype, int64_t rows, int64_t cols, int32_t n_z, double p,
+                                   uint64_t seed, uint64_t elem_offset, const uint64_t* state, int32_t draw, void* stream);
+
+/* h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight, row by row.  x, residual, h: (rows, cols) of `dtype` (F32, BF16,
+ * F16); residual and h are both given or both NULL (then h is x).  weight: (cols) floats or of `dtype`, NULL = ones.
+ * y_dtype = dtype: y is (rows, cols) of that type and scale is NULL.  y_dtype = CARD_DTYPE_E4M3: scale[row] = max |y| / 448
+ * (floats, (rows)) and y holds y / scale[row] in 8 bits; a row of zeros has scale 0, a row with a NaN is NaN throughout.
+ * y and scale come from h before h is rounded to its type.  cols <= CARD_NORM_MAX_COLS. */
+#define CARD_NORM_MAX_COLS 65536
+CARD_API int card_rms_norm(const void* x, const void* residual, const void* weight, int32_t dtype, int32_t weight_dtype, int64_t rows,
+                           int64_t cols, double eps, void* h, void* y, int32_t y_dtype, float* scale, void* stream);
+/* Gradients from h as the forward call stored it (x where there was no residual): g of y and gh of h (either NULL = zeros)
+ * give dx (the gradient of x and of the residual) and, unless NULL, dweight (of the weight's type).  dweight needs
+ * card_rms_norm_backward_workspace_bytes of scratch, 16-byte aligned; its sum over the rows has a fixed order. */
+CARD_API int card_rms_norm_backward_workspace_bytes(int32_t dtype, int64_t rows, int64_t cols, uint64_t* bytes);
+CARD_API int card_rms_norm_backward(const void* h, const void* weight, const void* g, const void* gh, int32_t dtype,
+                                    int32_t weight_dtype, int64_t rows, int64_t cols, double eps, void* dx, void* dweight,
+                                    void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* A Linear with 4-bit weights: w[o, k] = (q[o, k] - zero[o, k / group]) * scale[o, k / group].  Device pointers, copied into
+ * the kernel's layout at create time (on `stream`). */
+#define CARD_LINEAR4_MAX_FEATURES 1048576
+#define CARD_LINEAR4_MAX_ROWS 65535
+typedef struct card_linear4_desc {
+    int32_t struct_bytes;  /* sizeof(card_linear4_desc) */
+    int32_t in_features;
+    int32_t out_features;
+    int32_t group;         /* columns that share a scale: 32, 64 or 128 (the last group of a row may be shorter) */
+    const uint8_t* q;      /* (out, in): 0..15, one to a byte (the low four bits count) */
+    const float* scale;    /* (out, ceil(in / group)) */
+    const uint8_t* zero;   /* (out, ceil(in / group)): 0..15, or NULL = 8 everywhere */
+    const float* bias;     /* (out) or NULL */
+} card_linear4_desc;
+typedef struct card_linear4 card_linear4;
+CARD_API int card_linear4_create(const card_linear4_desc* desc, void* stream, card_linear4** out);
+CARD_API void card_linear4_destroy(card_linear4* s);
+/* y[m, o] = act(gamma[o] * (x_scale[m] * sum_k w[o, k] x[m, k] + bias[o])), act(v) = v > 0 ? v : slope * v.
+ * x (rows, in) of any card_dtype; x_scale (rows) goes with CARD_DTYPE_E4M3 and is NULL otherwise; gamma (out) or NULL = ones
+ * (a ConditionalLinear's embed.weight[t], regression/model.py:16-17); slope 1 = no activation; y (rows, out) F32, BF16 or F16.
+ * Made for one to some tens of rows; at most CARD_LINEAR4_MAX_ROWS.  The weights' device must be current. */
+CARD_API int card_linear4_forward(const card_linear4* s, const void* x, int32_t x_dtype, const float* x_scale, int64_t rows,
+                                  const float* gamma, float slope, void* y, int32_t y_dtype, void* stream);
+/* The nearest such weights of W (out, in) floats: per group scale = (max - min) / 15 over its values and 0, zero = round(-min /
+ * scale), q = round(w / scale) + zero.  q (out, in), scale and zero (out, ceil(in / group)). */
+CARD_API int card_linear4_quantize(const float* W, int32_t out_features, int32_t in_features, int32_t group, uint8_t* q, float* scale,
+                                   uint8_t* zero, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
