@@ -11,35 +11,49 @@
 using namespace card;
 
 struct card_linear4 {
-    int in, out, group, groups, device;
-    int words;                 // 32-bit words of a packed row: ceil(in / 8)
-    uint32_t* q;               // (out, words): nibble i of a word is column 8 * word + i
-    float* scale;              // (out, groups)
-    uint8_t* zero;             // (out, groups)
+    int in, out, group, device;
+    int blocks;                // blocks of kBlock columns: ceil(in / kBlock)
+    int tiles;                 // tiles of 16 outputs: ceil(out / 16)
+    uint4* q;                  // (tiles, blocks, 64): see pack_kernel
+    float* scale;              // (tiles, blocks, kBlock / group, 16)
+    uint8_t* zero;             // likewise, or NULL: 8 everywhere
     float* bias;               // (out)
 };
 
 namespace {
 
-constexpr int kThreads = 256, kRows = 8;
+constexpr int kThreads = 256, kBlock = 128, kMaxWaves = 8;
 
-__global__ void pack_kernel(const uint8_t* q, int in, int words, long long n, uint32_t* out) {
+// Weights in the order in which the matrix instruction takes them.  Of a tile of 16 outputs and a block of 128 columns lane l
+// holds 16 bytes: word s has the eight values of output l % 16 at the columns 32 s + 8 (l / 16) ... + 7 of the block.  The
+// value of column 2 j + h sits in the word's field j + 4 h; field 0 begins at bit 3 and field 7 wraps around.  A mask then
+// leaves two neighbouring columns as the mantissas of two bf16 numbers 16 + q (bf16_of below) and three shifts give the rest.
+__global__ void pack_kernel(const uint8_t* q, int in, int out_f, int blocks, long long n, uint4* out) {
     const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
     if (id >= n) return;
-    const long long o = id / words;
-    const int k = (int)(id - o * words) * 8;
-    uint32_t w = 0;
-    for (int i = 0; i < 8; ++i)
-        if (k + i < in) w |= (uint32_t)(q[o * in + k + i] & 15u) << (4 * i);
-    out[id] = w;
-}
-__global__ void side_kernel(const float* scale, const uint8_t* zero, const float* bias, long long n, int out_f, float* s, uint8_t* z, float* b) {
-    const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
-    if (id < n) {
-        s[id] = scale[id];
-        z[id] = zero ? zero[id] & 15u : 8u;
+    const int l = (int)(id & 63), block = (int)((id >> 6) % blocks);
+    const long long o = (id >> 6) / blocks * 16 + (l & 15);
+    uint32_t w[4];
+    for (int s = 0; s < 4; ++s) {
+        uint32_t u = 0;
+        for (int i = 0; i < 8; ++i) {
+            const int k = block * kBlock + 32 * s + 8 * (l >> 4) + i;
+            if (o < out_f && k < in) u |= (uint32_t)(q[o * in + k] & 15u) << (4 * (i / 2 + 4 * (i & 1)));
+        }
+        w[s] = u << 3 | u >> 29;
     }
+    out[id] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__global__ void side_kernel(const float* scale, const uint8_t* zero, const float* bias, int group, int groups, int blocks, int out_f,
+                            long long n, float* s, uint8_t* z, float* b) {
+    const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
     if (id < out_f) b[id] = bias ? bias[id] : 0.0f;
+    if (id >= n) return;
+    const int per = kBlock / group;
+    const long long at = id >> 4, o = at / per / blocks * 16 + (id & 15), g = at % ((long long)per * blocks);
+    const bool real = o < out_f && g < groups;
+    s[id] = real ? scale[o * groups + g] : 0.0f;
+    if (z) z[id] = real ? zero[o * groups + g] & 15u : 8u;
 }
 
 // one wave per (row o of the weights, group of columns): q = round(w / scale) + zero with scale = (max - min) / 15 over the
@@ -61,63 +75,263 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const float* W, int 
 }
 
 struct Args {
-    const uint32_t* q;
+    const uint4* q;
     const float* scale;
     const uint8_t* zero;
     const float* bias;
     const float* x_scale;
     const float* gamma;
     float slope;
-    int in, out, group, groups, words;
+    int in, out, blocks, tiles;
     int rows;
+    int per_wave;              // blocks of columns that a wave takes
+    int y_dtype;
 };
 
-__device__ __forceinline__ float e4m3_at(const uint8_t* p) { return __builtin_amdgcn_cvt_f32_fp8((int)*p, 0); }
-__device__ __forceinline__ float as_float(const float* p) { return *p; }
-__device__ __forceinline__ float as_float(const bf16_t* p) { return (float)*p; }
-__device__ __forceinline__ float as_float(const f16_t* p) { return (float)*p; }
-__device__ __forceinline__ float as_float(const uint8_t* p) { return e4m3_at(p); }
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// one wave per output column and kRows rows of x
-template <typename X, typename Y>
-__global__ __launch_bounds__(kThreads) void linear4_kernel(const Args a, const X* x, Y* y) {
-    const int o = blockIdx.x * (kThreads / 64) + threadIdx.x / 64, lane = threadIdx.x & 63, m0 = blockIdx.y * kRows;
-    if (o >= a.out) return;
-    float acc[kRows] = {};
-    for (int w = lane; w < a.words; w += 64) {
-        const uint32_t q = a.q[(long long)o * a.words + w];
-        const long long g = (long long)o * a.groups + w * 8 / a.group;
-        const float s = a.scale[g], z = a.zero[g];
+// eight 4-bit values as 16 + q, in bf16 (exponent of 16, q in mantissa bits 3-6) or fp16 (bits 6-9): no conversion, and exact
+template <int X> __device__ __forceinline__ u32x4 ints_of(uint32_t w) {
+    if constexpr (X == CARD_DTYPE_F16) {
+        const uint32_t m = 0x03C003C0u, c = 0x4C004C00u;
+        return u32x4{(__builtin_amdgcn_alignbit(w, w, 29) & m) | c, ((w >> 1) & m) | c, ((w >> 5) & m) | c, (__builtin_amdgcn_alignbit(w, w, 9) & m) | c};
+    } else {
+        const uint32_t m = 0x00780078u, c = 0x41804180u;
+        return u32x4{(w & m) | c, ((w >> 4) & m) | c, ((w >> 8) & m) | c, (__builtin_amdgcn_alignbit(w, w, 12) & m) | c};
+    }
+}
+template <int X> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (X == CARD_DTYPE_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// eight values of x as they lie in memory, and as operands: one of 16 bits each, or for fp32 three bf16 operands whose sum is
+// exactly x (8 + 8 + 8 of its 24 significant bits)
+template <int X> struct Row8;
+template <> struct Row8<CARD_DTYPE_BF16> {
+    typedef uint16_t elem;
+    static constexpr int kParts = 1, kWords = 4;
+};
+template <> struct Row8<CARD_DTYPE_F16> {
+    typedef uint16_t elem;
+    static constexpr int kParts = 1, kWords = 4;
+};
+template <> struct Row8<CARD_DTYPE_F32> {
+    typedef uint32_t elem;
+    static constexpr int kParts = 3, kWords = 8;
+};
+template <> struct Row8<CARD_DTYPE_E4M3> {
+    typedef uint8_t elem;
+    static constexpr int kParts = 1, kWords = 2;
+};
+template <int X> struct Raw { uint32_t w[Row8<X>::kWords]; };
+
+template <int X, bool TAIL> __device__ __forceinline__ Raw<X> load_x(const typename Row8<X>::elem* p, int left) {
+    typedef typename Row8<X>::elem E;
+    Raw<X> r;
+    if constexpr (!TAIL) {
+        typedef uint32_t words __attribute__((ext_vector_type(Row8<X>::kWords)));
+        typedef words loose __attribute__((aligned(sizeof(E))));
+        const words v = *reinterpret_cast<const loose*>(p);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (w * 8 + i >= a.in) break;
-            const float v = ((float)((q >> (4 * i)) & 15u) - z) * s;
+        for (int i = 0; i < Row8<X>::kWords; ++i) r.w[i] = v[i];
+    } else {
+        constexpr int per = 4 / sizeof(E);
 #pragma unroll
-            for (int m = 0; m < kRows; ++m)
-                if (m0 + m < a.rows) acc[m] += v * as_float(x + (long long)(m0 + m) * a.in + w * 8 + i);
+        for (int i = 0; i < Row8<X>::kWords; ++i) {
+            uint32_t v = 0;
+#pragma unroll
+            for (int j = 0; j < per; ++j)
+                if (i * per + j < left) v |= (uint32_t)p[i * per + j] << (j * 8 * sizeof(E) % 32);
+            r.w[i] = v;
+        }
+    }
+    return r;
+}
+template <int X> __device__ __forceinline__ void parts_of(const Raw<X>& r, u32x4 (&a)[Row8<X>::kParts]) {
+    if constexpr (X == CARD_DTYPE_F32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t h[2], m[2], l[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float v = __uint_as_float(r.w[2 * j + i]);
+                h[i] = r.w[2 * j + i] & 0xFFFF0000u;
+                const float v1 = v - __uint_as_float(h[i]);
+                m[i] = __float_as_uint(v1) & 0xFFFF0000u;
+                l[i] = __float_as_uint(v1 - __uint_as_float(m[i]));
+            }
+            a[0][j] = h[0] >> 16 | h[1];
+            a[1][j] = m[0] >> 16 | m[1];
+            a[2][j] = l[0] >> 16 | (l[1] & 0xFFFF0000u);
+        }
+    } else if constexpr (X == CARD_DTYPE_E4M3) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            a[0][2 * j] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.w[j], 1.0f, false));
+            a[0][2 * j + 1] = __builtin_bit_cast(uint32_t, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.w[j], 1.0f, true));
+        }
+    } else {
+        a[0] = u32x4{r.w[0], r.w[1], r.w[2], r.w[3]};
+    }
+}
+
+// One workgroup: 16 MT rows of x by 16 NT outputs; its waves share the blocks of columns and join through LDS in a fixed order.
+// Per group of columns the matrix pipe forms P = sum (16 + q) x and, against ones, S = sum x (shared by the NT tiles); the
+// vector pipe adds scale * (P - (16 + zero) S) to the fp32 sums.  Rows behind the last one repeat it and are not stored.
+// U blocks are on their way while one is used.
+template <int X, int G, int MT, int NT, int U>
+__global__ __launch_bounds__(64 * kMaxWaves) void linear4_kernel(const Args a, const typename Row8<X>::elem* x, void* y) {
+    typedef typename Row8<X>::elem E;
+    constexpr int P = Row8<X>::kParts;
+    extern __shared__ float join[];                  // (waves, MT * NT, 4, 64)
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
+    const int b0 = wave * a.per_wave, b1 = b0 + a.per_wave < a.blocks ? b0 + a.per_wave : a.blocks;
+    const E* xr[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = m0 + 16 * m + (lane & 15);
+        xr[m] = x + (long long)(row < a.rows ? row : a.rows - 1) * a.in + 8 * (lane >> 4);
+    }
+    long long tile_at[NT];                           // a tile behind the last one repeats it and is not stored
+#pragma unroll
+    for (int t = 0; t < NT; ++t) tile_at[t] = (long long)(tile0 + t < a.tiles ? tile0 + t : a.tiles - 1) * a.blocks;
+    struct Stage {
+        uint4 q[NT];
+        float s[NT][G];
+        uint32_t z[NT][G];
+        Raw<X> x[MT][4];
+    } st[U];
+    auto fetch = [&](Stage& g, int b) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const long long at = tile_at[t] + b;
+            g.q[t] = a.q[at * 64 + lane];
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                g.s[t][i] = a.scale[(at * G + i) * 16 + (lane & 15)];
+                g.z[t][i] = a.zero ? a.zero[(at * G + i) * 16 + (lane & 15)] : 8u;
+            }
+        }
+        if ((b + 1) * kBlock <= a.in) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) g.x[m][s] = load_x<X, false>(xr[m] + b * kBlock + 32 * s, 8);
+        } else {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) g.x[m][s] = load_x<X, true>(xr[m] + b * kBlock + 32 * s, a.in - (b * kBlock + 32 * s + 8 * (lane >> 4)));
+        }
+    };
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0, 0, 0, 0};
+    const uint32_t one = X == CARD_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
+    const u32x4 ones = {one, one, one, one};
+    auto use = [&](const Stage& g) {
+        constexpr int S = 4 / G;                     // steps of 32 columns in a group
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            f32x4 sum[MT], prod[MT][NT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                sum[m] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) prod[m][t] = f32x4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int s = i * S; s < (i + 1) * S; ++s) {
+                u32x4 w[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) w[t] = ints_of<X>(s == 0 ? g.q[t].x : s == 1 ? g.q[t].y : s == 2 ? g.q[t].z : g.q[t].w);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    u32x4 p[P];
+                    parts_of<X>(g.x[m][s], p);
+#pragma unroll
+                    for (int k = P - 1; k >= 0; --k) {          // the small parts first
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) prod[m][t] = mfma<X>(p[k], w[t], prod[m][t]);
+                        sum[m] = mfma<X>(p[k], ones, sum[m]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float off = -16.0f - (float)g.z[t][i], sc = g.s[t][i];
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(sc, fmaf(off, sum[m][r], prod[m][t][r]), acc[m][t][r]);
+            }
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (b0 + u < b1) fetch(st[u], b0 + u);
+    for (int b = b0; b < b1; b += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (b + u < b1) {
+                use(st[u]);
+                if (b + u + U < b1) fetch(st[u], b + u + U);
+            }
         }
     }
 #pragma unroll
-    for (int m = 0; m < kRows; ++m)
-        for (int s = 1; s < 64; s <<= 1) acc[m] += __shfl_xor(acc[m], s, 64);
-    if (lane) return;
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int m = 0; m < kRows; ++m) {
-        if (m0 + m >= a.rows) continue;
-        float v = (a.x_scale ? acc[m] * a.x_scale[m0 + m] : acc[m]) + a.bias[o];
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) join[((wave * MT * NT + m * NT + t) * 4 + r) * 64 + lane] = acc[m][t][r];
+    __syncthreads();
+    for (int id = threadIdx.x; id < MT * NT * 256; id += blockDim.x) {
+        const int l = id & 63, r = (id >> 6) & 3, t = (id >> 8) % NT, m = (id >> 8) / NT;
+        const int row = m0 + 16 * m + 4 * (l >> 4) + r;
+        const long long o = (long long)(tile0 + t) * 16 + (l & 15);
+        if (row >= a.rows || o >= a.out) continue;
+        float v = join[id];
+        for (int w = 1; w < waves; ++w) v += join[w * MT * NT * 256 + id];
+        if (a.x_scale) v *= a.x_scale[row];
+        v += a.bias[o];
         if (a.gamma) v *= a.gamma[o];
-        y[(long long)(m0 + m) * a.out + o] = (Y)(v > 0.0f ? v : v * a.slope);
+        v = v > 0.0f ? v : v * a.slope;
+        const long long at = (long long)row * a.out + o;
+        if (a.y_dtype == CARD_DTYPE_F32) ((float*)y)[at] = v;
+        else if (a.y_dtype == CARD_DTYPE_BF16) ((bf16_t*)y)[at] = (bf16_t)v;
+        else ((f16_t*)y)[at] = (f16_t)v;
     }
 }
 
-template <typename X, typename Y> int launch(const Args& a, const void* x, void* y, hipStream_t st) {
-    linear4_kernel<X, Y><<<dim3((a.out + 3) / 4, (a.rows + kRows - 1) / kRows), kThreads, 0, st>>>(a, (const X*)x, (Y*)y);
+template <int X, int G, int MT, int NT, int U> int launch(Args a, const void* x, void* y, hipStream_t st) {
+    // a wave takes four blocks of columns or more, so that its loads overlap; the split goes by the weights' shape alone: a row
+    // has the same bits however many rows come with it
+    int waves = 1;
+    while (waves < kMaxWaves && a.blocks >= 8 * waves) waves *= 2;
+    a.per_wave = (a.blocks + waves - 1) / waves;
+    const dim3 grid((a.tiles + NT - 1) / NT, (a.rows + 16 * MT - 1) / (16 * MT));
+    linear4_kernel<X, G, MT, NT, U><<<grid, 64 * waves, waves * MT * NT * 256 * sizeof(float), st>>>(a, (const typename Row8<X>::elem*)x, y);
     HIP_TRY(hipGetLastError());
     return CARD_OK;
 }
-template <typename X> int by_y(const Args& a, const void* x, void* y, int y_dtype, hipStream_t st) {
-    return y_dtype == CARD_DTYPE_F32 ? launch<X, float>(a, x, y, st) : y_dtype == CARD_DTYPE_BF16 ? launch<X, bf16_t>(a, x, y, st)
-                                                                                                 : launch<X, f16_t>(a, x, y, st);
+template <int X, int G> int by_rows(const Args& a, const void* x, void* y, hipStream_t st) {
+    constexpr int U = X == CARD_DTYPE_F32 ? 2 : 4;
+    if (a.rows <= 16) return a.tiles >= 1024 ? launch<X, G, 1, 2, U>(a, x, y, st) : launch<X, G, 1, 1, U>(a, x, y, st);
+    if (a.rows <= 32) return launch<X, G, 2, 2, 2>(a, x, y, st);
+    return launch<X, G, 4, 2, 1>(a, x, y, st);
+}
+template <int X> int by_group(const Args& a, int group, const void* x, void* y, hipStream_t st) {
+    return group == 128 ? by_rows<X, 1>(a, x, y, st) : group == 64 ? by_rows<X, 2>(a, x, y, st) : by_rows<X, 4>(a, x, y, st);
 }
 
 }  // namespace
@@ -150,18 +364,20 @@ extern "C" CARD_API int card_linear4_create(const card_linear4_desc* d, void* st
     if (!d->q || !d->scale) return card_fail(CARD_E_INVALID, "%s: null q / scale", who);
     card_linear4* s = new (std::nothrow) card_linear4();
     if (!s) return card_fail(CARD_E_NOMEM, "%s: out of host memory", who);
-    s->in = d->in_features; s->out = d->out_features; s->group = d->group; s->groups = (s->in + s->group - 1) / s->group;
-    s->words = (s->in + 7) / 8;
+    s->in = d->in_features; s->out = d->out_features; s->group = d->group;
+    s->blocks = (s->in + kBlock - 1) / kBlock; s->tiles = (s->out + 15) / 16;
     hipStream_t st = (hipStream_t)stream;
-    const long long nw = (long long)s->out * s->words, ng = (long long)s->out * s->groups;
+    const long long nw = (long long)s->tiles * s->blocks * 64, ng = (long long)s->tiles * s->blocks * (kBlock / s->group) * 16;
     hipError_t e = hipGetDevice(&s->device);
-    if (e == hipSuccess) e = hipMalloc(&s->q, nw * sizeof(uint32_t));
+    if (e == hipSuccess) e = hipMalloc(&s->q, nw * sizeof(uint4));
     if (e == hipSuccess) e = hipMalloc(&s->scale, ng * sizeof(float));
-    if (e == hipSuccess) e = hipMalloc(&s->zero, ng);
+    if (e == hipSuccess && d->zero) e = hipMalloc(&s->zero, ng);
     if (e == hipSuccess) e = hipMalloc(&s->bias, s->out * sizeof(float));
     if (e == hipSuccess) {
-        pack_kernel<<<(unsigned)((nw + kThreads - 1) / kThreads), kThreads, 0, st>>>(d->q, s->in, s->words, nw, s->q);
-        side_kernel<<<(unsigned)((ng + kThreads - 1) / kThreads), kThreads, 0, st>>>(d->scale, d->zero, d->bias, ng, s->out, s->scale, s->zero, s->bias);
+        const long long ns = ng > s->out ? ng : s->out;
+        pack_kernel<<<(unsigned)((nw + kThreads - 1) / kThreads), kThreads, 0, st>>>(d->q, s->in, s->out, s->blocks, nw, s->q);
+        side_kernel<<<(unsigned)((ns + kThreads - 1) / kThreads), kThreads, 0, st>>>(d->scale, d->zero, d->bias, s->group, (s->in + s->group - 1) / s->group,
+                                                                                  s->blocks, s->out, ng, s->scale, s->zero, s->bias);
         e = hipGetLastError();
     }
     if (e != hipSuccess) {
@@ -199,12 +415,12 @@ extern "C" CARD_API int card_linear4_forward(const card_linear4* s, const void* 
     if (device != s->device) return card_fail(CARD_E_INVALID, "%s: the weights are on device %d, the current device is %d", who, s->device, device);
     Args a;
     a.q = s->q; a.scale = s->scale; a.zero = s->zero; a.bias = s->bias; a.x_scale = x_scale; a.gamma = gamma; a.slope = slope;
-    a.in = s->in; a.out = s->out; a.group = s->group; a.groups = s->groups; a.words = s->words; a.rows = (int)rows;
+    a.in = s->in; a.out = s->out; a.blocks = s->blocks; a.tiles = s->tiles; a.rows = (int)rows; a.per_wave = 0; a.y_dtype = y_dtype;
     hipStream_t st = (hipStream_t)stream;
     switch (x_dtype) {
-        case CARD_DTYPE_F32: return by_y<float>(a, x, y, y_dtype, st);
-        case CARD_DTYPE_BF16: return by_y<bf16_t>(a, x, y, y_dtype, st);
-        case CARD_DTYPE_F16: return by_y<f16_t>(a, x, y, y_dtype, st);
-        default: return by_y<uint8_t>(a, x, y, y_dtype, st);
+        case CARD_DTYPE_F32: return by_group<CARD_DTYPE_F32>(a, s->group, x, y, st);
+        case CARD_DTYPE_BF16: return by_group<CARD_DTYPE_BF16>(a, s->group, x, y, st);
+        case CARD_DTYPE_F16: return by_group<CARD_DTYPE_F16>(a, s->group, x, y, st);
+        default: return by_group<CARD_DTYPE_E4M3>(a, s->group, x, y, st);
     }
 }
