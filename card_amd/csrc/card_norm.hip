@@ -5,9 +5,12 @@
 //   backward, from the h that forward stored:  gw = g * w,  dx = rstd * (gw - h * rstd^2 * mean(gw * h)) + gh,
 //   dw = sum over rows of g * h * rstd;  the residual's gradient is dx.
 //
-// Everything between a load and a store is 32 bits (rows of at most 64 columns: 64 bits in backward, see there); h and y are
-// rounded once, and y comes from the h that is not rounded yet.  A row is read once and lives in registers: V vectors of
-// 16 bytes in each of TPR threads.
+// Everything between a load and a store is 32 bits (rows of at most 8 vectors: 64 bits in backward, see there); h and y are
+// rounded once, and y comes from the h that is not rounded yet.
+//
+// What bounds it is memory: a row is read once and lives in registers, V vectors of 16 bytes in each thread of a workgroup
+// of as many waves as the row needs (up to 64 vectors: one wave, up to 8: eight lanes).  A workgroup walks over rows with the
+// weight in registers and asks for the next row before it joins the sums of this one, so loads are on their way all the time.
 #include "card_layers.h"
 
 using namespace card;
@@ -38,20 +41,37 @@ __device__ __forceinline__ float max_nan(float a, float b) {          // for val
     return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
 }
 
-// all-reduce over the TPR threads of a row; `buf` holds two floats per wave of the workgroup's row, `turn` alternates
-template <int TPR, typename F, typename Op> __device__ __forceinline__ F row_reduce(F v, F* buf, Op op) {
+// all-reduce over the threads of a row: L lanes of a wave, or (L = 0) the workgroup through `buf`, 16 floats that are not
+// written again before another barrier
+template <int L, typename F, typename Op> __device__ __forceinline__ F row_reduce(F v, F* buf, Op op) {
 #pragma unroll
-    for (int o = 1; o < (TPR < 64 ? TPR : 64); o <<= 1) v = op(v, __shfl_xor(v, o, 64));
-    if constexpr (TPR > 64) {
-        constexpr int W = TPR / 64;
+    for (int o = 1; o < (L ? L : 64); o <<= 1) v = op(v, __shfl_xor(v, o, 64));
+    if constexpr (L == 0) {
         if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
         __syncthreads();
         v = buf[0];
-#pragma unroll
-        for (int k = 1; k < W; ++k) v = op(v, buf[k]);
+        for (int k = 1; k < (int)(blockDim.x >> 6); ++k) v = op(v, buf[k]);
     }
     return v;
 }
+
+// a thread's vectors of one row as they lie in memory
+template <typename T, int V> struct RowRaw {
+    typename Vec<T, 16 / sizeof(T)>::type v[V];
+    __device__ __forceinline__ void load(const T* row, int cols, int t, int threads, bool live) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (k * threads + t) * N, n = live ? cols - c : 0;
+            if (n >= N) {
+                v[k] = *reinterpret_cast<const typename Vec<T, N>::loose*>(row + c);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) v[k][i] = i < n ? row[c + i] : (T)0.0f;
+            }
+        }
+    }
+};
 
 template <int N, typename T> __device__ __forceinline__ void load_w(const NormArgs& a, int c, int n, float (&w)[N]) {
     if (!a.w) {
@@ -70,40 +90,55 @@ __device__ __forceinline__ int pack_e4m3(float a, float b, float c, float d) {
     return __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
 
-template <typename T, int TPR, int V, bool Q>
-__global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads) void rms_norm_kernel(const NormArgs a) {
-    constexpr int N = 16 / sizeof(T), T_WG = TPR > kThreads ? TPR : kThreads, RPW = T_WG / TPR;
-    __shared__ float buf[2][TPR > 64 ? TPR / 64 : 1];
-    const int t = threadIdx.x % TPR;
-    for (long long r0 = (long long)blockIdx.x * RPW; r0 < a.rows; r0 += (long long)gridDim.x * RPW) {
-        const long long row = r0 + threadIdx.x / TPR;
+// L lanes per row (0: the workgroup), V vectors per thread
+template <typename T, int L, int V, bool Q>
+__global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_kernel(const NormArgs a) {
+    constexpr int N = 16 / sizeof(T);
+    constexpr bool kAhead = V <= 2;                       // longer rows fill the registers by themselves
+    __shared__ float buf[2][2][16];
+    const int threads = L ? L : blockDim.x, t = L ? threadIdx.x % L : threadIdx.x, rpw = L ? kThreads / L : 1;
+    const long long step = (long long)gridDim.x * rpw;
+    long long row = (long long)blockIdx.x * rpw + (L ? threadIdx.x / L : 0);
+    const long long last = L ? (a.rows + rpw - 1) / rpw * rpw : a.rows;          // all lanes of a wave take the same number of turns
+    float w[V][N];
+    if constexpr (kAhead) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) load_w<N, T>(a, (v * threads + t) * N, a.cols - (v * threads + t) * N, w[v]);
+    }
+    RowRaw<T, V> x, r;
+    auto fetch = [&](long long at) {
+        x.load((const T*)a.x + at * a.cols, a.cols, t, threads, at < a.rows);
+        if (a.residual) r.load((const T*)a.residual + at * a.cols, a.cols, t, threads, at < a.rows);
+    };
+    if (kAhead && row < last) fetch(row);
+    for (int turn = 0; row < last; row += step, turn ^= 1) {
         const bool live = row < a.rows;
+        if constexpr (!kAhead) fetch(row);
         float h[V][N];
         float ss = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int c = (v * TPR + t) * N, n = live ? a.cols - c : 0;
-            load_n<N>((const T*)a.x + row * a.cols + c, n, h[v]);
-            if (a.residual) {
-                float r[N];
-                load_n<N>((const T*)a.residual + row * a.cols + c, n, r);
+            const int c = (v * threads + t) * N, n = live ? a.cols - c : 0;
 #pragma unroll
-                for (int i = 0; i < N; ++i) h[v][i] += r[i];
+            for (int i = 0; i < N; ++i) h[v][i] = (float)x.v[v][i];
+            if (a.residual) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) h[v][i] += (float)r.v[v][i];
                 if (n > 0) store_n<N>((T*)a.h + row * a.cols + c, n, h[v]);
             }
 #pragma unroll
             for (int i = 0; i < N; ++i) ss += h[v][i] * h[v][i];
         }
-        ss = row_reduce<TPR>(ss, buf[0], [](float p, float q) { return p + q; });
+        if (kAhead && row + step < last) fetch(row + step);
+        ss = row_reduce<L>(ss, buf[turn][0], [](float p, float q) { return p + q; });
         const float rstd = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
         float amax = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int c = (v * TPR + t) * N, n = live ? a.cols - c : 0;
-            float w[N];
-            load_w<N, T>(a, c, n, w);
+            const int c = (v * threads + t) * N, n = live ? a.cols - c : 0;
+            if constexpr (!kAhead) load_w<N, T>(a, c, n, w[v]);
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[v][i] = h[v][i] * rstd * w[i];
+            for (int i = 0; i < N; ++i) h[v][i] = h[v][i] * rstd * w[v][i];
             if constexpr (Q) {
 #pragma unroll
                 for (int i = 0; i < N; ++i)
@@ -113,13 +148,13 @@ __global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads) void rms_norm_kern
             }
         }
         if constexpr (Q) {
-            amax = row_reduce<TPR>(amax, buf[1], max_nan);
+            amax = row_reduce<L>(amax, buf[turn][1], max_nan);
             // a row of zeros (or of values below 448 / FLT_MAX) must not divide by zero; NaN stays NaN
             const float inv = amax < 1.4e-36f ? 3.0e38f : kE4m3Max / amax;
             if (live && t == 0) a.scale[row] = amax / kE4m3Max;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const int c = (v * TPR + t) * N, n = live ? a.cols - c : 0;
+                const int c = (v * threads + t) * N, n = live ? a.cols - c : 0;
                 unsigned char* q = (unsigned char*)a.y + row * a.cols + c;
                 int word[N / 4];
 #pragma unroll
@@ -134,120 +169,164 @@ __global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads) void rms_norm_kern
                 }
             }
         }
-        if constexpr (TPR > 64) __syncthreads();            // buf is free for the next row
     }
 }
 
 // F: in rows of a few columns the two terms of dx all but cancel (at one column to eps * rstd^2 of either), so there the
 // row's numbers and the difference are formed in 64 bits.
-template <typename T, typename F, int TPR, int V>
-__global__ __launch_bounds__(TPR > kThreads ? TPR : kThreads) void rms_norm_backward_kernel(const NormArgs a) {
-    constexpr int N = 16 / sizeof(T), T_WG = TPR > kThreads ? TPR : kThreads, RPW = T_WG / TPR;
-    __shared__ F buf[2][TPR > 64 ? TPR / 64 : 1];
-    __shared__ float join[RPW > 1 ? RPW * TPR * V * N : 1];
-    const int t = threadIdx.x % TPR;
-    float dw[V][N] = {};
-    for (long long r0 = (long long)blockIdx.x * RPW; r0 < a.rows; r0 += (long long)gridDim.x * RPW) {
-        const long long row = r0 + threadIdx.x / TPR;
+template <typename T, typename F, int L, int V>
+__global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_backward_kernel(const NormArgs a) {
+    constexpr int N = 16 / sizeof(T), RPW = L ? kThreads / L : 1;
+    constexpr bool kAhead = V <= 2;
+    __shared__ F buf[2][2][16];
+    __shared__ float join[L ? RPW * L * V * N : 1];
+    const int threads = L ? L : blockDim.x, t = L ? threadIdx.x % L : threadIdx.x;
+    const long long step = (long long)gridDim.x * RPW;
+    long long row = (long long)blockIdx.x * RPW + (L ? threadIdx.x / L : 0);
+    const long long last = L ? (a.rows + RPW - 1) / RPW * RPW : a.rows;
+    float w[V][N], dw[V][N] = {};
+    if constexpr (kAhead) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) load_w<N, T>(a, (v * threads + t) * N, a.cols - (v * threads + t) * N, w[v]);
+    }
+    RowRaw<T, V> rh, rg, rgh;
+    auto fetch = [&](long long at) {
+        rh.load((const T*)a.x + at * a.cols, a.cols, t, threads, at < a.rows);
+        rg.load((const T*)a.g + at * a.cols, a.cols, t, threads, a.g && at < a.rows);
+        rgh.load((const T*)a.gh + at * a.cols, a.cols, t, threads, a.gh && at < a.rows);
+    };
+    if (kAhead && row < last) fetch(row);
+    for (int turn = 0; row < last; row += step, turn ^= 1) {
         const bool live = row < a.rows;
-        float h[V][N], g[V][N];
+        if constexpr (!kAhead) fetch(row);
+        const RowRaw<T, V> h = rh, g = rg, gh = rgh;
         F ss = 0, sg = 0;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int c = (v * TPR + t) * N, n = live ? a.cols - c : 0;
-            float w[N];
-            load_n<N>((const T*)a.x + row * a.cols + c, n, h[v]);
-            load_n<N>((const T*)a.g + row * a.cols + c, a.g ? n : 0, g[v]);
-            load_w<N, T>(a, c, n, w);
+            if constexpr (!kAhead) load_w<N, T>(a, (v * threads + t) * N, a.cols - (v * threads + t) * N, w[v]);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                ss += (F)h[v][i] * h[v][i];
-                sg += (F)g[v][i] * w[i] * h[v][i];
+                const F hv = (F)(float)h.v[v][i];
+                ss += hv * hv;
+                sg += (F)(float)g.v[v][i] * w[v][i] * hv;
             }
         }
-        auto add = [](F p, F q) { return p + q; };
-        ss = row_reduce<TPR>(ss, buf[0], add);
-        sg = row_reduce<TPR>(sg, buf[1], add);
+        if (kAhead && row + step < last) fetch(row + step);
+#pragma unroll
+        for (int o = 1; o < (L ? L : 64); o <<= 1) {
+            ss += __shfl_xor(ss, o, 64);
+            sg += __shfl_xor(sg, o, 64);
+        }
+        if constexpr (L == 0) {                           // both sums behind one barrier; the other turn's buffers are free by then
+            if ((threadIdx.x & 63) == 0) {
+                buf[turn][0][threadIdx.x >> 6] = ss;
+                buf[turn][1][threadIdx.x >> 6] = sg;
+            }
+            __syncthreads();
+            ss = buf[turn][0][0];
+            sg = buf[turn][1][0];
+            for (int k = 1; k < (int)(blockDim.x >> 6); ++k) {
+                ss += buf[turn][0][k];
+                sg += buf[turn][1][k];
+            }
+        }
         const F rstd2 = (F)1 / (ss / (F)a.cols + (F)a.eps), rstd = sqrt(rstd2), k = rstd2 * sg / (F)a.cols;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int c = (v * TPR + t) * N, n = live ? a.cols - c : 0;
-            float w[N], gh[N], d[N];
-            load_w<N, T>(a, c, n, w);
-            load_n<N>((const T*)a.gh + row * a.cols + c, a.gh ? n : 0, gh);
+            const int c = (v * threads + t) * N, n = live ? a.cols - c : 0;
+            if constexpr (!kAhead) load_w<N, T>(a, c, n, w[v]);
+            float d[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                d[i] = (float)(rstd * ((F)g[v][i] * w[i] - h[v][i] * k) + gh[i]);
-                dw[v][i] += g[v][i] * (float)(h[v][i] * rstd);
+                const float hv = (float)h.v[v][i], gv = (float)g.v[v][i];
+                d[i] = (float)(rstd * ((F)gv * w[v][i] - hv * k) + (F)(float)gh.v[v][i]);
+                dw[v][i] += gv * (float)(hv * rstd);
             }
             if (n > 0) store_n<N>((T*)a.y + row * a.cols + c, n, d);
         }
-        if constexpr (TPR > 64) __syncthreads();
     }
     if (!a.part) return;
     float* part = a.part + (long long)blockIdx.x * a.cols;
-    if constexpr (RPW > 1) {             // the rows of a workgroup join before they leave it
-        constexpr int L = TPR * V * N;
+    if constexpr (L != 0) {              // the rows of a workgroup join before they leave it
+        constexpr int S = L * V * N;
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-            for (int i = 0; i < N; ++i) join[(threadIdx.x / TPR) * L + (v * TPR + t) * N + i] = dw[v][i];
+            for (int i = 0; i < N; ++i) join[(threadIdx.x / L) * S + (v * L + t) * N + i] = dw[v][i];
         __syncthreads();
-        for (int c = threadIdx.x; c < a.cols; c += T_WG) {
+        for (int c = threadIdx.x; c < a.cols; c += kThreads) {
             float s = 0.0f;
-            for (int k = 0; k < RPW; ++k) s += join[k * L + c];
+            for (int k = 0; k < RPW; ++k) s += join[k * S + c];
             part[c] = s;
         }
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int c = (v * TPR + t) * N;
+            const int c = (v * threads + t) * N;
             if (c < a.cols) store_n<N>(part + c, a.cols - c, dw[v]);
         }
     }
 }
 
-// dw[c] = sum of n partial rows, four threads a column, joined in a fixed order
-__global__ __launch_bounds__(kThreads) void dw_join_kernel(const float* part, int n, int cols, float* dw32, void* dw16, int bf16) {
-    __shared__ float s[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6;
-    float v = 0.0f;
-    if (c < cols)
-        for (int i = k; i < n; i += 4) v += part[(long long)i * cols + c];
-    s[k][threadIdx.x & 63] = v;
+// dw[c] = sum of n partial rows: 32 columns to a workgroup, 8 lanes of four columns, the rows over the other 128 threads;
+// a fixed order throughout
+constexpr int kJoinCols = 32, kJoinThreads = 1024;
+__global__ __launch_bounds__(kJoinThreads) void dw_join_kernel(const float* part, int n, int cols, float* dw32, void* dw16, int bf16) {
+    constexpr int R = kJoinThreads / 8;
+    __shared__ float s[R][kJoinCols + 1];
+    const int lane = threadIdx.x & 7, k = threadIdx.x >> 3, c = blockIdx.x * kJoinCols + lane * 4;
+    float v[4] = {};
+    for (int i = k; i < n; i += R) {
+        float p[4];
+        load_n<4>(part + (long long)i * cols + c, cols - c, p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += p[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[k][lane * 4 + j] = v[j];
     __syncthreads();
-    if (k || c >= cols) return;
-    v = (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]);
-    if (dw32) dw32[c] = v;
-    else if (bf16) ((bf16_t*)dw16)[c] = (bf16_t)v;
-    else ((f16_t*)dw16)[c] = (f16_t)v;
+    const int col = threadIdx.x & 31, q = threadIdx.x >> 5;          // 32 threads per column, four partial sums each
+    float sum = (s[q][col] + s[q + 32][col]) + (s[q + 64][col] + s[q + 96][col]);
+    __syncthreads();
+    s[q][col] = sum;
+    __syncthreads();
+    if (q || blockIdx.x * kJoinCols + col >= cols) return;
+#pragma unroll
+    for (int j = 1; j < 32; ++j) sum += s[j][col];
+    const int o = blockIdx.x * kJoinCols + col;
+    if (dw32) dw32[o] = sum;
+    else if (bf16) ((bf16_t*)dw16)[o] = (bf16_t)sum;
+    else ((f16_t*)dw16)[o] = (f16_t)sum;
 }
 
 constexpr int kMaxCols = CARD_NORM_MAX_COLS;
-constexpr int kBackwardGroups = 1024;      // at most so many partial rows of dw
+constexpr int kGroups = 512;               // workgroups that walk over rows: two of up to 1024 threads on each of 256 CUs
+constexpr int kSmallGroups = 2048;         // ... of 256 threads
 
-struct Form { int tpr, v; };               // threads per row, vectors per thread: the smallest that holds a row
+struct Form { int lanes, v, threads; };    // lanes per row (0: a workgroup of `threads`), vectors per thread
 Form form_of(int64_t cols, int n) {
-    const int64_t vecs = (cols + n - 1) / n;
-    const Form all[] = {{8, 1}, {64, 1}, {64, 2}, {256, 1}, {256, 2}, {256, 4}, {1024, 2}, {1024, 4}, {1024, 8}, {1024, 16}};
-    for (const Form& f : all)
-        if ((int64_t)f.tpr * f.v >= vecs) return f;
-    return {0, 0};
+    const int vecs = (int)((cols + n - 1) / n);
+    if (vecs <= 8) return {8, 1, kThreads};
+    if (vecs <= 64) return {64, 1, kThreads};
+    int v = 1;
+    while ((int64_t)v * 1024 < vecs) v *= 2;
+    const int waves = (vecs + 64 * v - 1) / (64 * v);
+    return {0, v, 64 * waves};
 }
-long long groups(const Form& f, int64_t rows, long long most) {
-    const long long rpw = f.tpr < kThreads ? kThreads / f.tpr : 1, g = (rows + rpw - 1) / rpw;
+long long groups(const Form& f, int64_t rows) {
+    const long long rpw = f.lanes ? kThreads / f.lanes : 1, g = (rows + rpw - 1) / rpw;
+    const long long most = f.threads > kThreads ? kGroups : kSmallGroups;
     return g < most ? g : most;
 }
 
 template <typename T, bool Q> int forward(const NormArgs& a, hipStream_t st) {
     constexpr int N = 16 / sizeof(T);
     const Form f = form_of(a.cols, N);
-    const unsigned grid = (unsigned)groups(f, a.rows, 1 << 20);
-#define CARD_NORM_CASE(TPR, V) \
-    if (f.tpr == TPR && f.v == V) rms_norm_kernel<T, TPR, V, Q><<<grid, TPR > kThreads ? TPR : kThreads, 0, st>>>(a)
-    CARD_NORM_CASE(8, 1); CARD_NORM_CASE(64, 1); CARD_NORM_CASE(64, 2); CARD_NORM_CASE(256, 1); CARD_NORM_CASE(256, 2);
-    CARD_NORM_CASE(256, 4); CARD_NORM_CASE(1024, 2); CARD_NORM_CASE(1024, 4); CARD_NORM_CASE(1024, 8);
-    if constexpr (sizeof(T) == 4) CARD_NORM_CASE(1024, 16);
+    const unsigned grid = (unsigned)groups(f, a.rows);
+#define CARD_NORM_CASE(L, V) \
+    if (f.lanes == L && f.v == V) rms_norm_kernel<T, L, V, Q><<<grid, f.threads, 0, st>>>(a)
+    CARD_NORM_CASE(8, 1); CARD_NORM_CASE(64, 1); CARD_NORM_CASE(0, 1); CARD_NORM_CASE(0, 2); CARD_NORM_CASE(0, 4); CARD_NORM_CASE(0, 8);
+    if constexpr (sizeof(T) == 4) CARD_NORM_CASE(0, 16);
 #undef CARD_NORM_CASE
     HIP_TRY(hipGetLastError());
     return CARD_OK;
@@ -256,13 +335,12 @@ template <typename T, bool Q> int forward(const NormArgs& a, hipStream_t st) {
 template <typename T> int backward(const NormArgs& a, hipStream_t st) {
     constexpr int N = 16 / sizeof(T);
     const Form f = form_of(a.cols, N);
-    const unsigned grid = (unsigned)groups(f, a.rows, kBackwardGroups);
-#define CARD_NORM_CASE(F, TPR, V) \
-    if (f.tpr == TPR && f.v == V) rms_norm_backward_kernel<T, F, TPR, V><<<grid, TPR > kThreads ? TPR : kThreads, 0, st>>>(a)
-    CARD_NORM_CASE(double, 8, 1); CARD_NORM_CASE(float, 64, 1); CARD_NORM_CASE(float, 64, 2); CARD_NORM_CASE(float, 256, 1);
-    CARD_NORM_CASE(float, 256, 2); CARD_NORM_CASE(float, 256, 4); CARD_NORM_CASE(float, 1024, 2); CARD_NORM_CASE(float, 1024, 4);
-    CARD_NORM_CASE(float, 1024, 8);
-    if constexpr (sizeof(T) == 4) CARD_NORM_CASE(float, 1024, 16);
+    const unsigned grid = (unsigned)groups(f, a.rows);
+#define CARD_NORM_CASE(F, L, V) \
+    if (f.lanes == L && f.v == V) rms_norm_backward_kernel<T, F, L, V><<<grid, f.threads, 0, st>>>(a)
+    CARD_NORM_CASE(double, 8, 1); CARD_NORM_CASE(float, 64, 1); CARD_NORM_CASE(float, 0, 1); CARD_NORM_CASE(float, 0, 2);
+    CARD_NORM_CASE(float, 0, 4); CARD_NORM_CASE(float, 0, 8);
+    if constexpr (sizeof(T) == 4) CARD_NORM_CASE(float, 0, 16);
 #undef CARD_NORM_CASE
     HIP_TRY(hipGetLastError());
     return CARD_OK;
@@ -306,7 +384,7 @@ extern "C" CARD_API int card_rms_norm_backward_workspace_bytes(int32_t dtype, in
     const int rc = check("card_rms_norm_backward_workspace_bytes", dtype, dtype, rows, cols, 0.0);
     if (rc != CARD_OK) return rc;
     if (!bytes) return card_fail(CARD_E_INVALID, "card_rms_norm_backward_workspace_bytes: null argument");
-    *bytes = (uint64_t)groups(form_of(cols, 16 / (int)card_dtype_bytes(dtype)), rows, kBackwardGroups) * (uint64_t)cols * sizeof(float);
+    *bytes = (uint64_t)groups(form_of(cols, 16 / (int)card_dtype_bytes(dtype)), rows) * (uint64_t)cols * sizeof(float);
     return CARD_OK;
 }
 
@@ -318,7 +396,7 @@ extern "C" CARD_API int card_rms_norm_backward(const void* h, const void* weight
     if (rc != CARD_OK) return rc;
     if (rows > 0 && (!h || !dx)) return card_fail(CARD_E_INVALID, "%s: null h / dx", who);
     if (dweight && !weight) return card_fail(CARD_E_INVALID, "%s: dweight without a weight", who);
-    const int n = (int)groups(form_of(cols, 16 / (int)card_dtype_bytes(dtype)), rows, kBackwardGroups);
+    const int n = (int)groups(form_of(cols, 16 / (int)card_dtype_bytes(dtype)), rows);
     if (dweight && rows > 0 && (!workspace || workspace_bytes < (uint64_t)n * (uint64_t)cols * sizeof(float)))
         return card_fail(CARD_E_INVALID, "%s: workspace of %llu bytes, need %llu", who, (unsigned long long)workspace_bytes,
                          (unsigned long long)((uint64_t)n * (uint64_t)cols * sizeof(float)));
@@ -334,7 +412,7 @@ extern "C" CARD_API int card_rms_norm_backward(const void* h, const void* weight
     }
     if (dweight) {
         const bool f32 = weight_dtype == CARD_DTYPE_F32;
-        dw_join_kernel<<<(unsigned)((cols + 63) / 64), kThreads, 0, st>>>((const float*)workspace, n, (int)cols, f32 ? (float*)dweight : nullptr,
+        dw_join_kernel<<<(unsigned)((cols + kJoinCols - 1) / kJoinCols), kJoinThreads, 0, st>>>((const float*)workspace, n, (int)cols, f32 ? (float*)dweight : nullptr,
                                                                          f32 ? nullptr : dweight, weight_dtype == CARD_DTYPE_BF16);
         HIP_TRY(hipGetLastError());
     }
