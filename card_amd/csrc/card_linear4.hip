@@ -16,7 +16,7 @@ struct card_linear4 {
     int tiles;                 // tiles of 16 outputs: ceil(out / 16)
     uint4* q;                  // (tiles, blocks, 64): see pack_kernel
     float* scale;              // (tiles, blocks, kBlock / group, 16)
-    uint8_t* zero;             // likewise, or NULL: 8 everywhere
+    uint8_t* zero;             // likewise
     float* bias;               // (out)
 };
 
@@ -53,7 +53,7 @@ __global__ void side_kernel(const float* scale, const uint8_t* zero, const float
     const long long at = id >> 4, o = at / per / blocks * 16 + (id & 15), g = at % ((long long)per * blocks);
     const bool real = o < out_f && g < groups;
     s[id] = real ? scale[o * groups + g] : 0.0f;
-    if (z) z[id] = real ? zero[o * groups + g] & 15u : 8u;
+    z[id] = real && zero ? zero[o * groups + g] & 15u : 8u;
 }
 
 // one wave per (row o of the weights, group of columns): q = round(w / scale) + zero with scale = (max - min) / 15 over the
@@ -84,7 +84,6 @@ struct Args {
     float slope;
     int in, out, blocks, tiles;
     int rows;
-    int per_wave;              // blocks of columns that a wave takes
     int y_dtype;
 };
 
@@ -92,14 +91,22 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// eight 4-bit values as 16 + q, in bf16 (exponent of 16, q in mantissa bits 3-6) or fp16 (bits 6-9): no conversion, and exact
-template <int X> __device__ __forceinline__ u32x4 ints_of(uint32_t w) {
+// eight 4-bit values as 16 + q, in bf16 (exponent of 16, q in mantissa bits 3-6) or fp16 (bits 6-9): no conversion, and exact.
+// `sixteen` holds the two exponents and comes from sixteen_of, in a vector register: an instruction takes one literal, and
+// with the mask as that one a word's pair is a single v_and_or_b32.
+template <int X> __device__ __forceinline__ uint32_t sixteen_of() {
+    uint32_t c;
+    asm("v_mov_b32 %0, %1" : "=v"(c) : "i"(X == CARD_DTYPE_F16 ? 0x4C004C00 : 0x41804180));
+    return c;
+}
+template <int X> __device__ __forceinline__ u32x4 ints_of(uint32_t w, uint32_t sixteen) {
     if constexpr (X == CARD_DTYPE_F16) {
-        const uint32_t m = 0x03C003C0u, c = 0x4C004C00u;
-        return u32x4{(__builtin_amdgcn_alignbit(w, w, 29) & m) | c, ((w >> 1) & m) | c, ((w >> 5) & m) | c, (__builtin_amdgcn_alignbit(w, w, 9) & m) | c};
+        const uint32_t m = 0x03C003C0u;
+        return u32x4{(__builtin_amdgcn_alignbit(w, w, 29) & m) | sixteen, ((w >> 1) & m) | sixteen, ((w >> 5) & m) | sixteen,
+                     (__builtin_amdgcn_alignbit(w, w, 9) & m) | sixteen};
     } else {
-        const uint32_t m = 0x00780078u, c = 0x41804180u;
-        return u32x4{(w & m) | c, ((w >> 4) & m) | c, ((w >> 8) & m) | c, (__builtin_amdgcn_alignbit(w, w, 12) & m) | c};
+        const uint32_t m = 0x00780078u;
+        return u32x4{(w & m) | sixteen, ((w >> 4) & m) | sixteen, ((w >> 8) & m) | sixteen, (__builtin_amdgcn_alignbit(w, w, 12) & m) | sixteen};
     }
 }
 template <int X> __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -181,154 +188,224 @@ template <int X> __device__ __forceinline__ void parts_of(const Raw<X>& r, u32x4
     }
 }
 
-// One workgroup: 16 MT rows of x by 16 NT outputs; its waves share the blocks of columns and join through LDS in a fixed order.
-// Per group of columns the matrix pipe forms P = sum (16 + q) x and, against ones, S = sum x (shared by the NT tiles); the
-// vector pipe adds scale * (P - (16 + zero) S) to the fp32 sums.  Rows behind the last one repeat it and are not stored.
-// U blocks are on their way while one is used.
-template <int X, int G, int MT, int NT, int U>
-__global__ __launch_bounds__(64 * kMaxWaves) void linear4_kernel(const Args a, const typename Row8<X>::elem* x, void* y) {
-    typedef typename Row8<X>::elem E;
-    constexpr int P = Row8<X>::kParts;
-    extern __shared__ float join[];                  // (waves, MT * NT, 4, 64)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
-    const int b0 = wave * a.per_wave, b1 = b0 + a.per_wave < a.blocks ? b0 + a.per_wave : a.blocks;
-    const E* xr[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int row = m0 + 16 * m + (lane & 15);
-        xr[m] = x + (long long)(row < a.rows ? row : a.rows - 1) * a.in + 8 * (lane >> 4);
-    }
-    long long tile_at[NT];                           // a tile behind the last one repeats it and is not stored
-#pragma unroll
-    for (int t = 0; t < NT; ++t) tile_at[t] = (long long)(tile0 + t < a.tiles ? tile0 + t : a.tiles - 1) * a.blocks;
-    struct Stage {
-        uint4 q[NT];
-        float s[NT][G];
-        uint32_t z[NT][G];
-        Raw<X> x[MT][4];
-    } st[U];
-    auto fetch = [&](Stage& g, int b) {
+// a block of weights of NT tiles on its way
+template <int G, int NT, bool STREAM> struct Weights {
+    u32x4 q[NT];
+    float s[NT][G];
+    uint32_t z[NT][G];
+    // at: the block's index, the same for all lanes
+    __device__ __forceinline__ void load(const Args& a, const long long (&at)[NT], int b) {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const long long at = tile_at[t] + b;
-            g.q[t] = a.q[at * 64 + lane];
+            const long long i = at[t] + b;
+            const u32x4* p = (const u32x4*)(a.q + i * 64) + lane;
+            q[t] = STREAM ? __builtin_nontemporal_load(p) : *p;
 #pragma unroll
-            for (int i = 0; i < G; ++i) {
-                g.s[t][i] = a.scale[(at * G + i) * 16 + (lane & 15)];
-                g.z[t][i] = a.zero ? a.zero[(at * G + i) * 16 + (lane & 15)] : 8u;
-            }
-        }
-        if ((b + 1) * kBlock <= a.in) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int s = 0; s < 4; ++s) g.x[m][s] = load_x<X, false>(xr[m] + b * kBlock + 32 * s, 8);
-        } else {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int s = 0; s < 4; ++s) g.x[m][s] = load_x<X, true>(xr[m] + b * kBlock + 32 * s, a.in - (b * kBlock + 32 * s + 8 * (lane >> 4)));
-        }
-    };
-    f32x4 acc[MT][NT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0, 0, 0, 0};
-    const uint32_t one = X == CARD_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
-    const u32x4 ones = {one, one, one, one};
-    auto use = [&](const Stage& g) {
-        constexpr int S = 4 / G;                     // steps of 32 columns in a group
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-            f32x4 sum[MT], prod[MT][NT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                sum[m] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int t = 0; t < NT; ++t) prod[m][t] = f32x4{0, 0, 0, 0};
-            }
-#pragma unroll
-            for (int s = i * S; s < (i + 1) * S; ++s) {
-                u32x4 w[NT];
-#pragma unroll
-                for (int t = 0; t < NT; ++t) w[t] = ints_of<X>(s == 0 ? g.q[t].x : s == 1 ? g.q[t].y : s == 2 ? g.q[t].z : g.q[t].w);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    u32x4 p[P];
-                    parts_of<X>(g.x[m][s], p);
-#pragma unroll
-                    for (int k = P - 1; k >= 0; --k) {          // the small parts first
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) prod[m][t] = mfma<X>(p[k], w[t], prod[m][t]);
-                        sum[m] = mfma<X>(p[k], ones, sum[m]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const float off = -16.0f - (float)g.z[t][i], sc = g.s[t][i];
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(sc, fmaf(off, sum[m][r], prod[m][t][r]), acc[m][t][r]);
-            }
-        }
-    };
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-        if (b0 + u < b1) fetch(st[u], b0 + u);
-    for (int b = b0; b < b1; b += U) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (b + u < b1) {
-                use(st[u]);
-                if (b + u + U < b1) fetch(st[u], b + u + U);
+            for (int g = 0; g < G; ++g) {
+                s[t][g] = (a.scale + (i * G + g) * 16)[lane & 15];
+                z[t][g] = (a.zero + (i * G + g) * 16)[lane & 15];
             }
         }
     }
+};
+
+// acc += one block: per group of columns the matrix pipe forms P = sum (16 + q) x and, against ones, S = sum x (for all NT
+// tiles), the vector pipe adds scale * (P - (16 + zero) S).  part(m, s, k): the k-th part of step s of rows 16 m ...
+template <int X, int G, int MT, int NT, bool STREAM, typename F>
+__device__ __forceinline__ void add_block(const Weights<G, NT, STREAM>& w, uint32_t sixteen, f32x4 (&acc)[MT][NT], F part) {
+    constexpr int P = Row8<X>::kParts, S = 4 / G;          // S steps of 32 columns in a group
+    const uint32_t one = X == CARD_DTYPE_F16 ? 0x3C003C00u : 0x3F803F80u;
+    const u32x4 ones = {one, one, one, one};
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        f32x4 sum[MT], prod[MT][NT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            sum[m] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < NT; ++t) prod[m][t] = f32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int s = g * S; s < (g + 1) * S; ++s) {
+            u32x4 v[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) v[t] = ints_of<X>(w.q[t][s], sixteen);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                u32x4 p[P];
+                part(m, s, p);
+#pragma unroll
+                for (int k = P - 1; k >= 0; --k) {          // the small parts first
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) prod[m][t] = mfma<X>(p[k], v[t], prod[m][t]);
+                    sum[m] = mfma<X>(p[k], ones, sum[m]);
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float off = -16.0f - (float)w.z[t][g], sc = w.s[t][g];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(sc, fmaf(off, sum[m][r], prod[m][t][r]), acc[m][t][r]);
+        }
+    }
+}
+
+// What the epilogue multiplies and adds for one output: asked for at the start, so that it has come by the end.
+struct Out {
+    int row;
+    long long o;
+    float x_scale, bias, gamma;
+    bool real;
+    template <int MT> __device__ __forceinline__ void ask(const Args& a, int id, int tile0, int m0) {
+        const int l = id & 63, r = (id >> 6) & 3, m = (id >> 8) % MT, t = (id >> 8) / MT;
+        row = m0 + 16 * m + 4 * (l >> 4) + r;
+        o = (long long)(tile0 + t) * 16 + (l & 15);
+        real = row < a.rows && o < a.out;
+        x_scale = real && a.x_scale ? a.x_scale[row] : 1.0f;
+        bias = real ? a.bias[o] : 0.0f;
+        gamma = real && a.gamma ? a.gamma[o] : 1.0f;
+    }
+};
+
+// The waves join through LDS in a fixed order, and the epilogue.
+template <int MT, int NT>
+__device__ __forceinline__ void finish(const Args& a, const f32x4 (&acc)[MT][NT], float* join, int tile0, int m0, Out out, void* y) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) join[((wave * MT * NT + m * NT + t) * 4 + r) * 64 + lane] = acc[m][t][r];
+            for (int r = 0; r < 4; ++r) join[((wave * NT + t) * MT + m) * 256 + r * 64 + lane] = acc[m][t][r];
     __syncthreads();
-    for (int id = threadIdx.x; id < MT * NT * 256; id += blockDim.x) {
-        const int l = id & 63, r = (id >> 6) & 3, t = (id >> 8) % NT, m = (id >> 8) / NT;
-        const int row = m0 + 16 * m + 4 * (l >> 4) + r;
-        const long long o = (long long)(tile0 + t) * 16 + (l & 15);
-        if (row >= a.rows || o >= a.out) continue;
+    constexpr int n = NT * MT * 256;
+    for (int id = threadIdx.x; id < n; id += blockDim.x) {
+        if (id >= (int)blockDim.x) out.ask<MT>(a, id, tile0, m0);
+        if (!out.real) continue;
         float v = join[id];
-        for (int w = 1; w < waves; ++w) v += join[w * MT * NT * 256 + id];
-        if (a.x_scale) v *= a.x_scale[row];
-        v += a.bias[o];
-        if (a.gamma) v *= a.gamma[o];
+        for (int w = 1; w < waves; ++w) v += join[w * n + id];
+        v = (v * out.x_scale + out.bias) * out.gamma;
         v = v > 0.0f ? v : v * a.slope;
-        const long long at = (long long)row * a.out + o;
+        const long long at = (long long)out.row * a.out + out.o;
         if (a.y_dtype == CARD_DTYPE_F32) ((float*)y)[at] = v;
         else if (a.y_dtype == CARD_DTYPE_BF16) ((bf16_t*)y)[at] = (bf16_t)v;
         else ((f16_t*)y)[at] = (f16_t)v;
     }
 }
 
-template <int X, int G, int MT, int NT, int U> int launch(Args a, const void* x, void* y, hipStream_t st) {
-    // a wave takes four blocks of columns or more, so that its loads overlap; the split goes by the weights' shape alone: a row
-    // has the same bits however many rows come with it
-    int waves = 1;
-    while (waves < kMaxWaves && a.blocks >= 8 * waves) waves *= 2;
-    a.per_wave = (a.blocks + waves - 1) / waves;
+// One workgroup: 16 MT rows of x by 16 NT outputs; each of its waves takes a run of blocks of columns.
+//
+// The matrix instruction wants row l % 16 of x in lane l.  Asked for like that, 16 neighbouring lanes read 16 rows and every
+// load costs 64 cycles of the cache's address path (42 us for 16 rows of 8192 columns, 28672 outputs, against 31.5).  So lane l
+// asks for row l / 4 -- four lanes share a row's 64 bytes -- and ds_bpermute hands the values over where they are used; LDS
+// between them took as long and needs barriers.  U blocks of weights and of x are on their way while one is used: the loop
+// over them has no branch, or every wait in it would be for all of them.  A last block that is not full comes after the loop.
+template <int X, int G, int MT, int NT, int U, bool STREAM>
+__global__ __launch_bounds__(64 * kMaxWaves) void linear4_kernel(const Args a, const typename Row8<X>::elem* x, void* y) {
+    extern __shared__ float join[];                  // (waves, NT, MT, 4, 64)
+    constexpr int W = Row8<X>::kWords;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
+    const int full = a.in / kBlock, b0 = full * wave / waves, b1 = full * (wave + 1) / waves;
+    const int lrow = lane >> 2, lcol = 8 * (lane & 3), from = 4 * (4 * (lane & 15) + (lane >> 4));
+    const typename Row8<X>::elem* xr[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int row = m0 + 16 * m + lrow;
+        xr[m] = x + (long long)(row < a.rows ? row : a.rows - 1) * a.in + lcol;
+    }
+    long long at[NT];                                // a tile behind the last one repeats it and is not stored
+#pragma unroll
+    for (int t = 0; t < NT; ++t) at[t] = (long long)(tile0 + t < a.tiles ? tile0 + t : a.tiles - 1) * a.blocks;
+    struct Stage {
+        Weights<G, NT, STREAM> w;
+        Raw<X> x[MT][4];
+    } st[U];
+    auto fetch = [&](Stage& g, int b) {
+        g.w.load(a, at, b);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) g.x[m][s] = load_x<X, false>(xr[m] + b * kBlock + 32 * s, 8);
+    };
+    Out out = {};
+    if (threadIdx.x < NT * MT * 256) out.ask<MT>(a, threadIdx.x, tile0, m0);
+    const uint32_t sixteen = sixteen_of<X>();
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0, 0, 0, 0};
+    auto use = [&](const Stage& g) {
+        add_block<X, G, MT, NT, STREAM>(g.w, sixteen, acc, [&](int m, int s, u32x4 (&p)[Row8<X>::kParts]) {
+            Raw<X> r = g.x[m][s];
+#pragma unroll
+            for (int i = 0; i < W; ++i) r.w[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)r.w[i]);
+            parts_of<X>(r, p);
+        });
+    };
+    int b = b0;
+    if (b1 - b0 >= 2 * U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) fetch(st[u], b + u);
+        for (; b + 2 * U <= b1; b += U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                use(st[u]);
+                fetch(st[u], b + u + U);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (b + u < b1) fetch(st[u], b + u);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (b + u < b1) use(st[u]);
+        if (b + u + U < b1) fetch(st[u], b + u + U);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (b + u + U < b1) use(st[u]);
+    if (full < a.blocks && wave == waves - 1) {
+        st[0].w.load(a, at, full);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) st[0].x[m][s] = load_x<X, true>(xr[m] + full * kBlock + 32 * s, a.in - (full * kBlock + 32 * s + lcol));
+        use(st[0]);
+    }
+    finish<MT, NT>(a, acc, join, tile0, m0, out, y);
+}
+
+template <int X, int G, int MT, int NT, int U, bool STREAM> int launch(const Args& a, const void* x, void* y, hipStream_t st) {
+    int waves = 1;                                   // a block of columns for each at least
+    while (waves < kMaxWaves && a.blocks >= 2 * waves) waves *= 2;
     const dim3 grid((a.tiles + NT - 1) / NT, (a.rows + 16 * MT - 1) / (16 * MT));
-    linear4_kernel<X, G, MT, NT, U><<<grid, 64 * waves, waves * MT * NT * 256 * sizeof(float), st>>>(a, (const typename Row8<X>::elem*)x, y);
+    linear4_kernel<X, G, MT, NT, U, STREAM><<<grid, 64 * waves, waves * NT * MT * 256 * sizeof(float), st>>>(a, (const typename Row8<X>::elem*)x, y);
     HIP_TRY(hipGetLastError());
     return CARD_OK;
 }
+// Several tiles share the values of x where there are more tiles than CUs (24 rows, 6144 outputs: 9.8 us with two against
+// 10.3).  From 1024 tiles on the weights pass by the caches, which cannot hold them (16 rows of 8192 columns, 28672 outputs:
+// 29.7 us against 31.5; but 5.8 against 5.1 for 4096 x 4096, whose weights stay in L2 from call to call), and there `wide`
+// rows -- more than 16, or fp32 with its three operands -- take four tiles and one block on its way in the registers that
+// hold two and two otherwise (8192 columns, 28672 outputs: 32 rows bf16 44 us against 50, 16 rows fp32 49 against 71; one row
+// bf16 31 against 28).
+constexpr int kCus = 256, kStreamTiles = 1024;
+template <int X, int G, int MT> int by_tiles(const Args& a, const void* x, void* y, hipStream_t st) {
+    constexpr bool wide = X == CARD_DTYPE_F32 || MT > 1;
+    constexpr int U = wide ? 1 : 2;
+    if (a.tiles <= kCus) return launch<X, G, MT, 1, U, false>(a, x, y, st);
+    return a.tiles < kStreamTiles ? launch<X, G, MT, 2, U, false>(a, x, y, st) : launch<X, G, MT, wide ? 4 : 2, U, true>(a, x, y, st);
+}
 template <int X, int G> int by_rows(const Args& a, const void* x, void* y, hipStream_t st) {
-    constexpr int U = X == CARD_DTYPE_F32 ? 2 : 4;
-    if (a.rows <= 16) return a.tiles >= 1024 ? launch<X, G, 1, 2, U>(a, x, y, st) : launch<X, G, 1, 1, U>(a, x, y, st);
-    if (a.rows <= 32) return launch<X, G, 2, 2, 2>(a, x, y, st);
-    return launch<X, G, 4, 2, 1>(a, x, y, st);
+    return a.rows <= 16 ? by_tiles<X, G, 1>(a, x, y, st) : by_tiles<X, G, 2>(a, x, y, st);
 }
 template <int X> int by_group(const Args& a, int group, const void* x, void* y, hipStream_t st) {
     return group == 128 ? by_rows<X, 1>(a, x, y, st) : group == 64 ? by_rows<X, 2>(a, x, y, st) : by_rows<X, 4>(a, x, y, st);
@@ -371,7 +448,7 @@ extern "C" CARD_API int card_linear4_create(const card_linear4_desc* d, void* st
     hipError_t e = hipGetDevice(&s->device);
     if (e == hipSuccess) e = hipMalloc(&s->q, nw * sizeof(uint4));
     if (e == hipSuccess) e = hipMalloc(&s->scale, ng * sizeof(float));
-    if (e == hipSuccess && d->zero) e = hipMalloc(&s->zero, ng);
+    if (e == hipSuccess) e = hipMalloc(&s->zero, ng);
     if (e == hipSuccess) e = hipMalloc(&s->bias, s->out * sizeof(float));
     if (e == hipSuccess) {
         const long long ns = ng > s->out ? ng : s->out;
@@ -415,7 +492,7 @@ extern "C" CARD_API int card_linear4_forward(const card_linear4* s, const void* 
     if (device != s->device) return card_fail(CARD_E_INVALID, "%s: the weights are on device %d, the current device is %d", who, s->device, device);
     Args a;
     a.q = s->q; a.scale = s->scale; a.zero = s->zero; a.bias = s->bias; a.x_scale = x_scale; a.gamma = gamma; a.slope = slope;
-    a.in = s->in; a.out = s->out; a.blocks = s->blocks; a.tiles = s->tiles; a.rows = (int)rows; a.per_wave = 0; a.y_dtype = y_dtype;
+    a.in = s->in; a.out = s->out; a.blocks = s->blocks; a.tiles = s->tiles; a.rows = (int)rows; a.y_dtype = y_dtype;
     hipStream_t st = (hipStream_t)stream;
     switch (x_dtype) {
         case CARD_DTYPE_F32: return by_group<CARD_DTYPE_F32>(a, s->group, x, y, st);
