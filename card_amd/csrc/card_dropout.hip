@@ -44,11 +44,10 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(const Shape s, const 
     float v[N], r[N];
     load_n<N>(x + from, n, v);
     if (residual) load_n<N>(residual + at, n, r);
-    const uint32_t m = keep_bits<N>(d, seed, off + (unsigned long long)at, n < N ? (int)n : N);
+    drop<N>(d, seed, off + (unsigned long long)at, n < N ? (int)n : N, v);
+    if (residual) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        v[i] = (m >> i) & 1 ? v[i] * d.scale : 0.0f;
-        if (residual) v[i] += r[i];
+        for (int i = 0; i < N; ++i) v[i] += r[i];
     }
     store_n<N>(out + at, n, v);
 }

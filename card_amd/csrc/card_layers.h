@@ -56,6 +56,25 @@ __device__ __forceinline__ void drop_key(const DropRule& d, unsigned long long& 
     seed = d.state ? d.state[0] : d.seed;
     off = d.elem_offset + (d.state ? d.state[1] : 0ull);
 }
+// Philox4x32-10 of the block (c, draw, 1): card_common.h's generator in 20 multiplies that give both halves and 20 three-way
+// xors; the keys are the same for all lanes and step on the scalar unit.  A stream of bf16 elements is bound by these
+// instructions and not by memory: 8192 x 4096, forward or backward, 43 us with two multiplies and two xors for one, 33 us so.
+__device__ __forceinline__ void drop_words(const DropRule& d, unsigned long long seed, unsigned long long c, uint32_t (&r)[4]) {
+    uint32_t c0 = (uint32_t)c, c1 = (uint32_t)(c >> 32), c2 = d.draw, c3 = 1u, k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+        unsigned long long p0, p1, cc;
+        asm("v_mad_u64_u32 %0, %1, %2, %3, 0" : "=v"(p0), "=s"(cc) : "v"(c0), "s"(0xD2511F53u));
+        asm("v_mad_u64_u32 %0, %1, %2, %3, 0" : "=v"(p1), "=s"(cc) : "v"(c2), "s"(0xCD9E8D57u));
+        const uint32_t h0 = (uint32_t)(p0 >> 32), l0 = (uint32_t)p0, h1 = (uint32_t)(p1 >> 32), l1 = (uint32_t)p1;
+        c0 = __builtin_amdgcn_bitop3_b32(h1, c1, k0, 0x96);
+        c2 = __builtin_amdgcn_bitop3_b32(h0, c3, k1, 0x96);
+        c1 = l1; c3 = l0;
+        k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
+    }
+    r[0] = c0; r[1] = c1; r[2] = c2; r[3] = c3;
+}
+
 // bit j: element e + j is kept, j < n <= N (bits from n on may be anything)
 template <int N>
 __device__ __forceinline__ uint32_t keep_bits(const DropRule& d, unsigned long long seed, unsigned long long e, int n) {
@@ -66,13 +85,28 @@ __device__ __forceinline__ uint32_t keep_bits(const DropRule& d, unsigned long l
     for (int k = 0; k <= N / 4; ++k) {
         if (4 * k < s + n) {
             uint32_t r[4];
-            const unsigned long long c = b + k;
-            philox4x32_10((uint32_t)c, (uint32_t)(c >> 32), d.draw, 1u, (uint32_t)seed, (uint32_t)(seed >> 32), r);
+            drop_words(d, seed, b + k, r);
 #pragma unroll
             for (int w = 0; w < 4; ++w) m |= (r[w] >= d.threshold ? 1u : 0u) << (4 * k + w);
         }
     }
     return d.none ? 0u : m >> s;
+}
+// v[j] = kept ? v[j] * scale : 0, for elements e ... e + N - 1
+template <int N> __device__ __forceinline__ void drop(const DropRule& d, unsigned long long seed, unsigned long long e, int n, float (&v)[N]) {
+    if ((e & 3) == 0 && !d.none) {                   // whole blocks: the words decide as they come
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k) {
+            uint32_t r[4];
+            drop_words(d, seed, (e >> 2) + k, r);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) v[4 * k + w] = r[w] >= d.threshold ? v[4 * k + w] * d.scale : 0.0f;
+        }
+    } else {
+        const uint32_t m = keep_bits<N>(d, seed, e, n);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (m >> i) & 1 ? v[i] * d.scale : 0.0f;
+    }
 }
 
 }  // namespace card
