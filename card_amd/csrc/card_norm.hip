@@ -41,18 +41,56 @@ __device__ __forceinline__ float max_nan(float a, float b) {          // for val
     return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
 }
 
+// v of the lane o away in the exchange that makes 2 o lanes alike once o are: quads by quad_perm, 8 and 16 lanes by mirrors,
+// 32 and 64 by swapping rows of lanes -- all on the vector unit, where a shuffle through LDS takes some 60 cycles a step
+template <int O> __device__ __forceinline__ float partner(float v) {
+    const int i = __builtin_bit_cast(int, v);
+    if constexpr (O == 1) return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0xB1, 0xF, 0xF, true));
+    else if constexpr (O == 2) return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0x4E, 0xF, 0xF, true));
+    else if constexpr (O == 4) return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0x141, 0xF, 0xF, true));
+    else return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(i, 0x140, 0xF, 0xF, true));
+}
+// the same value in all lanes of each group of L: op over the group
+template <int L, typename Op> __device__ __forceinline__ float lanes_reduce(float v, Op op) {
+    v = op(v, partner<1>(v));
+    v = op(v, partner<2>(v));
+    v = op(v, partner<4>(v));
+    if constexpr (L >= 16) v = op(v, partner<8>(v));
+    if constexpr (L >= 32) {
+        const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    }
+    if constexpr (L >= 64) {
+        const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    }
+    return v;
+}
+template <int L, typename Op> __device__ __forceinline__ double lanes_reduce(double v, Op op) {
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) v = op(v, __shfl_xor(v, o, 64));
+    return v;
+}
+// op over a workgroup's waves, whose values are in `buf` behind the barrier; absent waves hold 0 (clear_buf)
+template <typename Op> __device__ __forceinline__ float waves_reduce(const float* buf, Op op) {
+    return lanes_reduce<16>(buf[threadIdx.x & 15], op);
+}
 // all-reduce over the threads of a row: L lanes of a wave, or (L = 0) the workgroup through `buf`, 16 floats that are not
 // written again before another barrier
-template <int L, typename F, typename Op> __device__ __forceinline__ F row_reduce(F v, F* buf, Op op) {
-#pragma unroll
-    for (int o = 1; o < (L ? L : 64); o <<= 1) v = op(v, __shfl_xor(v, o, 64));
+template <int L, typename Op> __device__ __forceinline__ float row_reduce(float v, float* buf, Op op) {
+    v = lanes_reduce<L ? L : 64>(v, op);
     if constexpr (L == 0) {
         if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = buf[0];
-        for (int k = 1; k < (int)(blockDim.x >> 6); ++k) v = op(v, buf[k]);
+        v = waves_reduce(buf, op);
     }
     return v;
+}
+template <int L, int K> __device__ __forceinline__ void clear_buf(float (&buf)[K]) {
+    if constexpr (L == 0) {
+        if (threadIdx.x < K) buf[threadIdx.x] = 0.0f;          // a workgroup has K threads at least
+        __syncthreads();
+    }
 }
 
 // a thread's vectors of one row as they lie in memory
@@ -95,7 +133,9 @@ template <typename T, int L, int V, bool Q>
 __global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_kernel(const NormArgs a) {
     constexpr int N = 16 / sizeof(T);
     constexpr bool kAhead = V <= 2;                       // longer rows fill the registers by themselves
-    __shared__ float buf[2][2][16];
+    __shared__ __align__(16) float bufs[64];
+    float(*const buf)[2][16] = (float(*)[2][16])bufs;
+    clear_buf<L>(bufs);
     const int threads = L ? L : blockDim.x, t = L ? threadIdx.x % L : threadIdx.x, rpw = L ? kThreads / L : 1;
     const long long step = (long long)gridDim.x * rpw;
     long long row = (long long)blockIdx.x * rpw + (L ? threadIdx.x / L : 0);
@@ -113,17 +153,27 @@ __global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_kernel(const Nor
     if (kAhead && row < last) fetch(row);
     for (int turn = 0; row < last; row += step, turn ^= 1) {
         const bool live = row < a.rows;
-        if constexpr (!kAhead) fetch(row);
         float h[V][N];
         float ss = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int c = (v * threads + t) * N, n = live ? a.cols - c : 0;
+            if constexpr (kAhead) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[v][i] = (float)x.v[v][i];
+                for (int i = 0; i < N; ++i) h[v][i] = (float)x.v[v][i];
+            } else {
+                load_n<N>((const T*)a.x + row * a.cols + c, n, h[v]);
+            }
             if (a.residual) {
+                float rv[N];
+                if constexpr (kAhead) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) h[v][i] += (float)r.v[v][i];
+                    for (int i = 0; i < N; ++i) rv[i] = (float)r.v[v][i];
+                } else {
+                    load_n<N>((const T*)a.residual + row * a.cols + c, n, rv);
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) h[v][i] += rv[i];
                 if (n > 0) store_n<N>((T*)a.h + row * a.cols + c, n, h[v]);
             }
 #pragma unroll
@@ -172,38 +222,37 @@ __global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_kernel(const Nor
     }
 }
 
+// Six waves to a SIMD (80 registers) are worth more than the last registers: 40000 x 1000 bf16 71 us against 89.
 // F: in rows of a few columns the two terms of dx all but cancel (at one column to eps * rstd^2 of either), so there the
 // row's numbers and the difference are formed in 64 bits.
 template <typename T, typename F, int L, int V>
-__global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_backward_kernel(const NormArgs a) {
+__global__ __launch_bounds__(L ? kThreads : 1024, V == 1 && sizeof(F) == 4 ? 6 : 4) void rms_norm_backward_kernel(const NormArgs a) {
     constexpr int N = 16 / sizeof(T), RPW = L ? kThreads / L : 1;
-    constexpr bool kAhead = V <= 2;
-    __shared__ F buf[2][2][16];
+    static_assert(V <= 2, "longer rows: rms_norm_backward_long_kernel");
+    __shared__ __align__(16) float bufs[64];
+    float(*const buf)[2][16] = (float(*)[2][16])bufs;
+    clear_buf<L>(bufs);
     __shared__ float join[L ? RPW * L * V * N : 1];
     const int threads = L ? L : blockDim.x, t = L ? threadIdx.x % L : threadIdx.x;
     const long long step = (long long)gridDim.x * RPW;
     long long row = (long long)blockIdx.x * RPW + (L ? threadIdx.x / L : 0);
     const long long last = L ? (a.rows + RPW - 1) / RPW * RPW : a.rows;
     float w[V][N], dw[V][N] = {};
-    if constexpr (kAhead) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) load_w<N, T>(a, (v * threads + t) * N, a.cols - (v * threads + t) * N, w[v]);
-    }
+    for (int v = 0; v < V; ++v) load_w<N, T>(a, (v * threads + t) * N, a.cols - (v * threads + t) * N, w[v]);
     RowRaw<T, V> rh, rg, rgh;
     auto fetch = [&](long long at) {
         rh.load((const T*)a.x + at * a.cols, a.cols, t, threads, at < a.rows);
         rg.load((const T*)a.g + at * a.cols, a.cols, t, threads, a.g && at < a.rows);
         rgh.load((const T*)a.gh + at * a.cols, a.cols, t, threads, a.gh && at < a.rows);
     };
-    if (kAhead && row < last) fetch(row);
+    if (row < last) fetch(row);
     for (int turn = 0; row < last; row += step, turn ^= 1) {
         const bool live = row < a.rows;
-        if constexpr (!kAhead) fetch(row);
         const RowRaw<T, V> h = rh, g = rg, gh = rgh;
         F ss = 0, sg = 0;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            if constexpr (!kAhead) load_w<N, T>(a, (v * threads + t) * N, a.cols - (v * threads + t) * N, w[v]);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const F hv = (F)(float)h.v[v][i];
@@ -211,30 +260,23 @@ __global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_backward_kernel(
                 sg += (F)(float)g.v[v][i] * w[v][i] * hv;
             }
         }
-        if (kAhead && row + step < last) fetch(row + step);
-#pragma unroll
-        for (int o = 1; o < (L ? L : 64); o <<= 1) {
-            ss += __shfl_xor(ss, o, 64);
-            sg += __shfl_xor(sg, o, 64);
-        }
+        if (row + step < last) fetch(row + step);
+        auto add = [](F p, F q) { return p + q; };
+        ss = lanes_reduce<L ? L : 64>(ss, add);
+        sg = lanes_reduce<L ? L : 64>(sg, add);
         if constexpr (L == 0) {                           // both sums behind one barrier; the other turn's buffers are free by then
             if ((threadIdx.x & 63) == 0) {
                 buf[turn][0][threadIdx.x >> 6] = ss;
                 buf[turn][1][threadIdx.x >> 6] = sg;
             }
             __syncthreads();
-            ss = buf[turn][0][0];
-            sg = buf[turn][1][0];
-            for (int k = 1; k < (int)(blockDim.x >> 6); ++k) {
-                ss += buf[turn][0][k];
-                sg += buf[turn][1][k];
-            }
+            ss = waves_reduce(buf[turn][0], add);
+            sg = waves_reduce(buf[turn][1], add);
         }
         const F rstd2 = (F)1 / (ss / (F)a.cols + (F)a.eps), rstd = sqrt(rstd2), k = rstd2 * sg / (F)a.cols;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int c = (v * threads + t) * N, n = live ? a.cols - c : 0;
-            if constexpr (!kAhead) load_w<N, T>(a, c, n, w[v]);
             float d[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -264,6 +306,64 @@ __global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_backward_kernel(
         for (int v = 0; v < V; ++v) {
             const int c = (v * threads + t) * N;
             if (c < a.cols) store_n<N>(part + c, a.cols - c, dw[v]);
+        }
+    }
+}
+
+// Rows of more than 2 x 1024 vectors do not stay in registers: h and g are read again (from the caches, as far as they hold
+// them) once the row's sums are there, and the workgroup's partial dw lies in memory.
+template <typename T>
+__global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(const NormArgs a) {
+    constexpr int N = 16 / sizeof(T);
+    __shared__ __align__(16) float bufs[64];
+    float(*const buf)[2][16] = (float(*)[2][16])bufs;
+    clear_buf<0>(bufs);
+    float* const part = a.part ? a.part + (long long)blockIdx.x * a.cols : nullptr;
+    auto add = [](float p, float q) { return p + q; };
+    int turn = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const T *hr = (const T*)a.x + row * a.cols, *gr = (const T*)a.g + row * a.cols, *ghr = (const T*)a.gh + row * a.cols;
+        float ss = 0.0f, sg = 0.0f;
+#pragma unroll 2
+        for (int c = threadIdx.x * N; c < a.cols; c += 1024 * N) {
+            const int n = a.cols - c;
+            float h[N], g[N], w[N];
+            load_n<N>(hr + c, n, h);
+            load_n<N>(gr + c, a.g ? n : 0, g);
+            load_w<N, T>(a, c, n, w);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                ss += h[i] * h[i];
+                sg += g[i] * w[i] * h[i];
+            }
+        }
+        ss = lanes_reduce<64>(ss, add);
+        sg = lanes_reduce<64>(sg, add);
+        if ((threadIdx.x & 63) == 0) {
+            buf[turn][0][threadIdx.x >> 6] = ss;
+            buf[turn][1][threadIdx.x >> 6] = sg;
+        }
+        __syncthreads();
+        ss = waves_reduce(buf[turn][0], add);
+        sg = waves_reduce(buf[turn][1], add);
+        const float rstd2 = 1.0f / (ss / (float)a.cols + a.eps), rstd = sqrtf(rstd2), k = rstd2 * sg / (float)a.cols;
+#pragma unroll 2
+        for (int c = threadIdx.x * N; c < a.cols; c += 1024 * N) {
+            const int n = a.cols - c;
+            float h[N], g[N], w[N], gh[N], d[N];
+            load_n<N>(hr + c, n, h);
+            load_n<N>(gr + c, a.g ? n : 0, g);
+            load_n<N>(ghr + c, a.gh ? n : 0, gh);
+            load_w<N, T>(a, c, n, w);
+#pragma unroll
+            for (int i = 0; i < N; ++i) d[i] = rstd * (g[i] * w[i] - h[i] * k) + gh[i];
+            store_n<N>((T*)a.y + row * a.cols + c, n, d);
+            if (part) {
+                load_n<N>(part + c, row == blockIdx.x ? 0 : n, d);
+#pragma unroll
+                for (int i = 0; i < N; ++i) d[i] += g[i] * (h[i] * rstd);
+                store_n<N>(part + c, n, d);
+            }
         }
     }
 }
@@ -300,32 +400,38 @@ __global__ __launch_bounds__(kJoinThreads) void dw_join_kernel(const float* part
 }
 
 constexpr int kMaxCols = CARD_NORM_MAX_COLS;
-constexpr int kGroups = 512;               // workgroups that walk over rows: two of up to 1024 threads on each of 256 CUs
-constexpr int kSmallGroups = 2048;         // ... of 256 threads
+constexpr int kCus = 256;
+constexpr int kForwardWaves = 32, kBackwardWaves = 24;          // that a CU holds at a time: what the registers allow
 
 struct Form { int lanes, v, threads; };    // lanes per row (0: a workgroup of `threads`), vectors per thread
 Form form_of(int64_t cols, int n) {
     const int vecs = (int)((cols + n - 1) / n);
-    if (vecs <= 8) return {8, 1, kThreads};
-    if (vecs <= 64) return {64, 1, kThreads};
+    for (int lanes = 8; lanes <= 64; lanes *= 2)
+        if (vecs <= lanes) return {lanes, 1, kThreads};
     int v = 1;
     while ((int64_t)v * 1024 < vecs) v *= 2;
     const int waves = (vecs + 64 * v - 1) / (64 * v);
     return {0, v, 64 * waves};
 }
-long long groups(const Form& f, int64_t rows) {
-    const long long rpw = f.lanes ? kThreads / f.lanes : 1, g = (rows + rpw - 1) / rpw;
-    const long long most = f.threads > kThreads ? kGroups : kSmallGroups;
+// workgroups that walk over the rows: as many as the chip holds at a time
+long long groups(const Form& f, int64_t rows, int waves) {
+    const long long rpw = f.lanes ? kThreads / f.lanes : 1, g = (rows + rpw - 1) / rpw, per_cu = waves / (f.threads / 64);
+    const long long most = kCus * (per_cu > 0 ? per_cu : 1);
     return g < most ? g : most;
+}
+
+long long backward_groups(int32_t dtype, int64_t rows, int64_t cols) {
+    return groups(form_of(cols, 16 / (int)card_dtype_bytes(dtype)), rows, kBackwardWaves);
 }
 
 template <typename T, bool Q> int forward(const NormArgs& a, hipStream_t st) {
     constexpr int N = 16 / sizeof(T);
     const Form f = form_of(a.cols, N);
-    const unsigned grid = (unsigned)groups(f, a.rows);
+    const unsigned grid = (unsigned)groups(f, a.rows, kForwardWaves);
 #define CARD_NORM_CASE(L, V) \
     if (f.lanes == L && f.v == V) rms_norm_kernel<T, L, V, Q><<<grid, f.threads, 0, st>>>(a)
-    CARD_NORM_CASE(8, 1); CARD_NORM_CASE(64, 1); CARD_NORM_CASE(0, 1); CARD_NORM_CASE(0, 2); CARD_NORM_CASE(0, 4); CARD_NORM_CASE(0, 8);
+    CARD_NORM_CASE(8, 1); CARD_NORM_CASE(16, 1); CARD_NORM_CASE(32, 1); CARD_NORM_CASE(64, 1);
+    CARD_NORM_CASE(0, 1); CARD_NORM_CASE(0, 2); CARD_NORM_CASE(0, 4); CARD_NORM_CASE(0, 8);
     if constexpr (sizeof(T) == 4) CARD_NORM_CASE(0, 16);
 #undef CARD_NORM_CASE
     HIP_TRY(hipGetLastError());
@@ -335,12 +441,12 @@ template <typename T, bool Q> int forward(const NormArgs& a, hipStream_t st) {
 template <typename T> int backward(const NormArgs& a, hipStream_t st) {
     constexpr int N = 16 / sizeof(T);
     const Form f = form_of(a.cols, N);
-    const unsigned grid = (unsigned)groups(f, a.rows);
+    const unsigned grid = (unsigned)backward_groups(sizeof(T) == 4 ? CARD_DTYPE_F32 : CARD_DTYPE_BF16, a.rows, a.cols);
 #define CARD_NORM_CASE(F, L, V) \
     if (f.lanes == L && f.v == V) rms_norm_backward_kernel<T, F, L, V><<<grid, f.threads, 0, st>>>(a)
-    CARD_NORM_CASE(double, 8, 1); CARD_NORM_CASE(float, 64, 1); CARD_NORM_CASE(float, 0, 1); CARD_NORM_CASE(float, 0, 2);
-    CARD_NORM_CASE(float, 0, 4); CARD_NORM_CASE(float, 0, 8);
-    if constexpr (sizeof(T) == 4) CARD_NORM_CASE(float, 0, 16);
+    CARD_NORM_CASE(double, 8, 1); CARD_NORM_CASE(float, 16, 1); CARD_NORM_CASE(float, 32, 1); CARD_NORM_CASE(float, 64, 1);
+    CARD_NORM_CASE(float, 0, 1); CARD_NORM_CASE(float, 0, 2);
+    if (f.v > 2) rms_norm_backward_long_kernel<T><<<grid, 1024, 0, st>>>(a);
 #undef CARD_NORM_CASE
     HIP_TRY(hipGetLastError());
     return CARD_OK;
@@ -384,7 +490,7 @@ extern "C" CARD_API int card_rms_norm_backward_workspace_bytes(int32_t dtype, in
     const int rc = check("card_rms_norm_backward_workspace_bytes", dtype, dtype, rows, cols, 0.0);
     if (rc != CARD_OK) return rc;
     if (!bytes) return card_fail(CARD_E_INVALID, "card_rms_norm_backward_workspace_bytes: null argument");
-    *bytes = (uint64_t)groups(form_of(cols, 16 / (int)card_dtype_bytes(dtype)), rows) * (uint64_t)cols * sizeof(float);
+    *bytes = (uint64_t)backward_groups(dtype, rows, cols) * (uint64_t)cols * sizeof(float);
     return CARD_OK;
 }
 
@@ -396,7 +502,7 @@ extern "C" CARD_API int card_rms_norm_backward(const void* h, const void* weight
     if (rc != CARD_OK) return rc;
     if (rows > 0 && (!h || !dx)) return card_fail(CARD_E_INVALID, "%s: null h / dx", who);
     if (dweight && !weight) return card_fail(CARD_E_INVALID, "%s: dweight without a weight", who);
-    const int n = (int)groups(form_of(cols, 16 / (int)card_dtype_bytes(dtype)), rows);
+    const int n = (int)backward_groups(dtype, rows, cols);
     if (dweight && rows > 0 && (!workspace || workspace_bytes < (uint64_t)n * (uint64_t)cols * sizeof(float)))
         return card_fail(CARD_E_INVALID, "%s: workspace of %llu bytes, need %llu", who, (unsigned long long)workspace_bytes,
                          (unsigned long long)((uint64_t)n * (uint64_t)cols * sizeof(float)));
