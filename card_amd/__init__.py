@@ -20,7 +20,7 @@ from .diffusion_utils import (  # noqa: F401
     q_sample,
     y_0_reparam,
 )
-from .guidance import GuidanceNet, describe_guidance, guidance_for  # noqa: F401
+from .guidance import GuidanceNet, QuantGuidanceNet, describe_guidance, guidance_for  # noqa: F401
 from .layers import QuantLinear, dropout, quantize_weight, rms_norm, rms_norm_e4m3  # noqa: F401
 from .sampler import ModelDescription, Sampler, describe, invalidate, sampler_for, unwrap  # noqa: F401
 

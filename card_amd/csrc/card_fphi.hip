@@ -13,6 +13,7 @@
 #include <new>
 
 #include "card_internal.h"
+#include "card_layers.h"
 
 struct card_fphi {
     int n_layers;
@@ -49,8 +50,17 @@ __global__ void transpose_kernel(const float* __restrict__ W, int out_f, int in_
     Wt[(long long)k * out_f + o] = W[idx];
 }
 
-__global__ __launch_bounds__(kThreadsF) void fphi_forward_kernel(const FphiParams p, const float* __restrict__ x,
+// Monte-Carlo dropout: rows are chains, n_z of them to a row of x, and rule[l] drops the outputs of hidden layer l
+struct FphiMc {
+    int n_z;
+    card::DropRule rule[CARD_FPHI_MAX_LAYERS];
+};
+struct FphiNone {};
+
+template <typename MC>
+__global__ __launch_bounds__(kThreadsF) void fphi_forward_kernel(const FphiParams p, const MC mc, const float* __restrict__ x,
                                                                  long long rows, float* __restrict__ out) {
+    constexpr bool kMc = sizeof(MC) == sizeof(FphiMc);
     extern __shared__ __attribute__((aligned(16))) float act[];      // two [kRows][max_dim] activation buffers
     const int tid = threadIdx.x;
     const long long n_blocks = (rows + kRows - 1) / kRows;
@@ -60,7 +70,11 @@ __global__ __launch_bounds__(kThreadsF) void fphi_forward_kernel(const FphiParam
         float* cur = act;
         float* nxt = act + kRows * p.max_dim;
         const int d0 = p.dims[0];
-        for (int i = tid; i < nr * d0; i += kThreadsF) cur[i] = x[row0 * d0 + i];     // rows are contiguous: coalesced
+        if constexpr (kMc) {
+            for (int i = tid; i < nr * d0; i += kThreadsF) cur[i] = x[(row0 + i / d0) / mc.n_z * d0 + i % d0];
+        } else {
+            for (int i = tid; i < nr * d0; i += kThreadsF) cur[i] = x[row0 * d0 + i];     // rows are contiguous: coalesced
+        }
         __syncthreads();
         for (int l = 0; l < p.n_layers; ++l) {
             const int in_f = p.dims[l], out_f = p.dims[l + 1];
@@ -75,6 +89,11 @@ __global__ __launch_bounds__(kThreadsF) void fphi_forward_kernel(const FphiParam
                 if (!last) {
                     if (p.scale[l]) acc = acc * p.scale[l][o] + p.shift[l][o];         // eval-mode BatchNorm1d, model.py:74-75
                     acc = acc > 0.0f ? acc : acc * p.slope;                            // LeakyReLU, model.py:76
+                    if constexpr (kMc) {                                               // Dropout, model.py:77
+                        const card::DropRule& d = mc.rule[l];
+                        const uint32_t m = card::keep_bits<4>(d, d.seed, d.elem_offset + (unsigned long long)((row0 + r) * out_f + o), 1);
+                        acc = m & 1 ? acc * d.scale : 0.0f;
+                    }
                     nxt[r * out_f + o] = acc;
                 } else {
                     out[(row0 + r) * out_f + o] = acc;
@@ -150,7 +169,8 @@ extern "C" CARD_API void card_fphi_destroy(card_fphi* f) {
 int fphi_in_dim(const card_fphi* f) { return f->dims[0]; }
 int fphi_out_dim(const card_fphi* f) { return f->dims[f->n_layers]; }
 
-int fphi_forward(const card_fphi* f, const float* x, long long rows, float* out, hipStream_t stream) {
+namespace {
+template <typename MC> int run_fphi(const card_fphi* f, const MC& mc, const float* x, long long rows, float* out, hipStream_t stream) {
     FphiParams p;
     memset(&p, 0, sizeof(p));
     p.n_layers = f->n_layers; p.max_dim = f->max_dim; p.slope = f->slope;
@@ -161,9 +181,14 @@ int fphi_forward(const card_fphi* f, const float* x, long long rows, float* out,
     long long grid = (rows + kRows - 1) / kRows;
     if (grid > 8192) grid = 8192;
     const size_t lds = (size_t)2 * kRows * f->max_dim * sizeof(float);      // <= 64 KB at CARD_FPHI_MAX_WIDTH
-    fphi_forward_kernel<<<dim3((unsigned)grid), dim3(kThreadsF), lds, stream>>>(p, x, rows, out);
+    fphi_forward_kernel<MC><<<dim3((unsigned)grid), dim3(kThreadsF), lds, stream>>>(p, mc, x, rows, out);
     HIP_TRY(hipGetLastError());
     return CARD_OK;
+}
+}  // namespace
+
+int fphi_forward(const card_fphi* f, const float* x, long long rows, float* out, hipStream_t stream) {
+    return run_fphi(f, FphiNone(), x, rows, out, stream);
 }
 
 extern "C" CARD_API int card_fphi_forward(const card_fphi* f, const float* x, int64_t rows, float* out, void* stream) {
@@ -171,4 +196,23 @@ extern "C" CARD_API int card_fphi_forward(const card_fphi* f, const float* x, in
     if (rows == 0) return CARD_OK;
     if (!x || !out) return card_fail(CARD_E_INVALID, "card_fphi_forward: null x / out");
     return fphi_forward(f, x, rows, out, (hipStream_t)stream);
+}
+
+extern "C" CARD_API int card_fphi_forward_mc(const card_fphi* f, const float* x, int64_t rows, int32_t n_z, const double* p, uint64_t seed,
+                                             uint64_t chain_offset, float* out, void* stream) {
+    const char* who = "card_fphi_forward_mc";
+    if (!f || rows < 0 || n_z < 1) return card_fail(CARD_E_INVALID, "%s: null handle, rows=%lld < 0 or n_z=%d < 1", who, (long long)rows, n_z);
+    if (rows > INT64_MAX / 8 / CARD_FPHI_MAX_WIDTH / n_z) return card_fail(CARD_E_INVALID, "%s: more bytes than 63 bits count", who);
+    if (chain_offset > (uint64_t)INT64_MAX / CARD_FPHI_MAX_WIDTH) return card_fail(CARD_E_INVALID, "%s: chain_offset beyond 2^53", who);
+    if (!p && f->n_layers > 1) return card_fail(CARD_E_INVALID, "%s: null p", who);
+    FphiMc mc;
+    memset(&mc, 0, sizeof(mc));
+    mc.n_z = n_z;
+    for (int l = 0; l < f->n_layers - 1; ++l) {
+        const int rc = drop_rule(who, p[l], seed, chain_offset * (uint64_t)f->dims[l + 1], nullptr, l, &mc.rule[l]);
+        if (rc != CARD_OK) return rc;
+    }
+    if (rows == 0) return CARD_OK;
+    if (!x || !out) return card_fail(CARD_E_INVALID, "%s: null x / out", who);
+    return run_fphi(f, mc, x, rows * n_z, out, (hipStream_t)stream);
 }

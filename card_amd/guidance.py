@@ -17,9 +17,10 @@ from .sampler import _content_hash, _dev_f32, _fingerprint, _ptr, _require_cuda,
 
 
 class GuidanceNet:
-    """A packed f_phi on one GPU.  Immutable after construction."""
+    """A packed f_phi on one GPU.  Immutable after construction.  `dropout`: the rates of the hidden layers' Dropout, which
+    `mc_dropout` applies (`forward` is the eval-mode network)."""
 
-    def __init__(self, weights, biases, *, negative_slope=0.01, bn_scale=None, bn_shift=None, device):
+    def __init__(self, weights, biases, *, negative_slope=0.01, bn_scale=None, bn_shift=None, dropout=None, device):
         device = torch.device(device)
         _require_cuda(device)
         n = len(weights)
@@ -47,6 +48,7 @@ class GuidanceNet:
             if bn_scale is not None and bn_scale[l] is not None:
                 d.bn_scale[l], d.bn_shift[l] = dev(bn_scale[l]), dev(bn_shift[l])
         self.device, self.dim_in, self.dim_out = device, int(d.dims[0]), int(d.dims[n])
+        self.dropout = _rates(dropout, n)
         h = C.c_void_p()
         L = _lib.lib()
         with torch.cuda.device(device):
@@ -55,14 +57,23 @@ class GuidanceNet:
         weakref.finalize(self, L.card_fphi_destroy, h)
 
     @classmethod
-    def from_module(cls, net, device=None):
+    def from_module(cls, net, device=None, *, weight_bits=None, group=64):
         """From a DeterministicFeedForwardNeuralNetwork (its `.network` Sequential: Linear, [BatchNorm1d], LeakyReLU,
-        Dropout per hidden layer, then Linear -- regression/model.py:70-79) or any Sequential of those layer types."""
+        Dropout per hidden layer, then Linear -- regression/model.py:70-79) or any Sequential of those layer types.
+        weight_bits=4: the weights in 4 bits with a scale per `group` columns (QuantGuidanceNet); the layers may then be of
+        any width and may have an nn.RMSNorm ahead of them."""
         d = describe_guidance(net)
         device = device if device is not None else d["weights"][0].device
+        if weight_bits == 4:
+            return QuantGuidanceNet(d, group=group, device=device)
+        if weight_bits is not None:
+            raise CardError(f"f_phi: weight_bits={weight_bits}; 4, or None for fp32")
+        if any(n is not None for n in d["norms"]):
+            raise CardError("f_phi: RMSNorm layers run with weight_bits=4 only")
         sc = [None if bn is None else _bn_fold(bn)[0] for bn in d["batchnorm"]]
         sh = [None if bn is None else _bn_fold(bn)[1] for bn in d["batchnorm"]]
-        return cls(d["weights"], d["biases"], negative_slope=d["negative_slope"], bn_scale=sc, bn_shift=sh, device=device)
+        return cls(d["weights"], d["biases"], negative_slope=d["negative_slope"], bn_scale=sc, bn_shift=sh,
+                   dropout=d["dropout"], device=device)
 
     @classmethod
     def from_ols(cls, beta, device=None):
@@ -85,6 +96,117 @@ class GuidanceNet:
 
     __call__ = forward
 
+    def mc_dropout(self, x, n_z, *, seed, chain_offset=0):
+        """(rows, n_z, dim_out): the network with its Dropout layers active, n_z masks for every row (Monte-Carlo dropout):
+        card_fphi_forward_mc.  Hidden layer l drops what `card_amd.dropout(..., seed=seed, draw=l)` drops of its (rows * n_z,
+        width) outputs; chain_offset: the first row's number times n_z where rows are sharded."""
+        x, n_z, chain_offset = self._mc_args(x, n_z, chain_offset)
+        rows = int(x.shape[0])
+        out = torch.empty(rows, n_z, self.dim_out, device=self.device, dtype=torch.float32)
+        p = (C.c_double * max(1, len(self.dropout)))(*self.dropout)
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.lib().card_fphi_forward_mc(self._h, _ptr(x), rows, n_z, p, int(seed) & (2 ** 64 - 1), chain_offset,
+                                                       _ptr(out), _stream(self.device)), "card_fphi_forward_mc")
+        return out
+
+    def _rows(self, x):
+        x = _dev_f32(x, self.device)
+        if x.dim() != 2 or x.shape[1] != self.dim_in:
+            raise CardError(f"f_phi: x must be (rows, {self.dim_in}), got {tuple(x.shape)}")
+        return x
+
+    def _mc_args(self, x, n_z, chain_offset):
+        if self.dropout is None:
+            raise CardError("f_phi: no Dropout rates, or Dropout layers other than one behind each hidden layer")
+        x = self._rows(x)
+        if not 1 <= int(n_z) < 2 ** 31 or not 0 <= int(chain_offset) < 2 ** 52:
+            raise CardError(f"f_phi: n_z={n_z} or chain_offset={chain_offset} out of range")
+        return x, int(n_z), int(chain_offset)
+
+
+def _rates(dropout, n_layers):
+    if dropout is None:
+        return None
+    p = [float(v) for v in dropout]
+    if len(p) != n_layers - 1 or not all(0.0 <= v <= 1.0 for v in p):
+        raise CardError(f"f_phi: dropout rates {p} for {n_layers - 1} hidden layers")
+    return p
+
+
+class QuantGuidanceNet(GuidanceNet):
+    """f_phi with 4-bit weights: per layer [RMSNorm to e4m3 (card_rms_norm)], the 4-bit product with bias, folded BatchNorm and
+    LeakyReLU in its epilogue (card_linear4), and in `mc_dropout` the dropout (card_dropout).  Rows stay fp32 between layers,
+    8-bit behind a norm.  Where the sampler takes a GuidanceNet it takes this one; the network then runs ahead of the sampling
+    kernels instead of as their first."""
+
+    def __init__(self, description, *, group=64, device):
+        from .layers import QuantLinear
+        device = torch.device(device)
+        _require_cuda(device)
+        d = description
+        self.dim_in, self.dim_out = d["dims"][0], d["dims"][-1]
+        self.dropout, self.slope = _rates(d["dropout"], len(d["weights"])), d["negative_slope"]
+        self._h = None
+        self.layers = []
+        for W, b, bn, norm in zip(d["weights"], d["biases"], d["batchnorm"], d["norms"]):
+            W = _dev_f32(W, device)
+            b = _dev_f32(b, device) if b is not None else torch.zeros(W.shape[0], device=device)
+            if bn is not None:
+                sc, sh = (_dev_f32(t, device) for t in _bn_fold(bn))
+                W, b = W * sc[:, None], b * sc + sh
+            lin = QuantLinear.from_float(W, b, group=group, device=device)
+            w = None if norm is None or norm.weight is None else _dev_f32(norm.weight, device)
+            self.layers.append((norm is not None, w, 0.0 if norm is None else _eps(norm), lin))
+        self.device = self.layers[0][3].device
+
+    def _layer(self, l, h):
+        from .layers import rms_norm_e4m3
+        norm, w, eps, lin = self.layers[l]
+        scale = None
+        if norm:
+            h, scale = rms_norm_e4m3(h, w, eps=eps)
+        return lin.forward(h, scale, slope=self.slope if l < len(self.layers) - 1 else None, out_dtype=torch.float32)
+
+    def forward(self, x, out=None):
+        """(rows, dim_out) = f_phi(x)."""
+        h = self._rows(x)
+        with torch.no_grad():
+            h = torch.cat([self._part(h[i:i + _lib.LINEAR4_MAX_ROWS]) for i in range(0, h.shape[0], _lib.LINEAR4_MAX_ROWS)]) \
+                if h.shape[0] > _lib.LINEAR4_MAX_ROWS else self._part(h)
+            return h if out is None else out.copy_(h)
+
+    __call__ = forward
+
+    def _part(self, h):
+        for l in range(len(self.layers)):
+            h = self._layer(l, h)
+        return h
+
+    def mc_dropout(self, x, n_z, *, seed, chain_offset=0):
+        """GuidanceNet.mc_dropout with 4-bit weights: the same masks."""
+        from .layers import dropout
+        x, n_z, chain_offset = self._mc_args(x, n_z, chain_offset)
+        most = max(1, _lib.LINEAR4_MAX_ROWS // n_z)
+        if n_z > _lib.LINEAR4_MAX_ROWS:
+            raise CardError(f"f_phi: n_z={n_z} > {_lib.LINEAR4_MAX_ROWS} with 4-bit weights")
+        parts = []
+        with torch.no_grad():
+            for i in range(0, max(1, x.shape[0]), most):
+                h = x[i:i + most]
+                rows, chains, first = int(h.shape[0]), 1, chain_offset + i * n_z
+                for l in range(len(self.layers)):
+                    h = self._layer(l, h)
+                    # rows become chains at the first layer that drops something; the layers ahead of it run once per row
+                    if l < len(self.dropout) and self.dropout[l] > 0:
+                        z, chains = (n_z, n_z) if chains == 1 else (1, chains)
+                        h = dropout(h, self.dropout[l], seed=seed, elem_offset=first * h.shape[1], draw=l, n_z=z).reshape(rows * n_z, h.shape[1])
+                parts.append(h.reshape(rows, chains, self.dim_out).expand(rows, n_z, self.dim_out))
+        return parts[0].contiguous() if len(parts) == 1 else torch.cat(parts)
+
+
+def _eps(norm):
+    return torch.finfo(torch.float32).eps if norm.eps is None else float(norm.eps)
+
 
 def _bn_fold(m):
     """eval-mode BatchNorm1d as (scale, shift) per feature"""
@@ -95,42 +217,65 @@ def _bn_fold(m):
 def describe_guidance(net):
     """Recognise f_phi (device-free, like card_amd.sampler.describe): walk the `.network` Sequential of a
     DeterministicFeedForwardNeuralNetwork (regression/model.py:70-79) -- or any Sequential of Linear / BatchNorm1d /
-    LeakyReLU / ReLU / Dropout / Identity -- and return {"dims": [dim_in, hidden..., dim_out], "weights": [Linear.weight
-    ...], "biases": [...], "batchnorm": [the BatchNorm1d module that follows layer l, or None], "negative_slope": float}
+    LeakyReLU / ReLU / Dropout / RMSNorm / Identity -- and return {"dims": [dim_in, hidden..., dim_out], "weights": [Linear.weight
+    ...], "biases": [...], "batchnorm": [the BatchNorm1d module that follows layer l, or None], "negative_slope": float,
+    "dropout": [the Dropout rate behind hidden layer l] (None: Dropout layers elsewhere), "norms": [the RMSNorm ahead of layer l, or None]}
     with the module's own Parameter objects.  Raises CardError for train-mode BatchNorm / Dropout and foreign layers."""
     import torch.nn as nn
     net = getattr(net, "module", net) if isinstance(net, (nn.DataParallel, nn.parallel.DistributedDataParallel)) else net
     seq = getattr(net, "network", net)
     Ws, bs, bns, slope = [], [], [], None
+    drops, norms, norm, active, simple = [], [], None, False, True
     for m in seq.children():
         if isinstance(m, nn.Linear):
             Ws.append(m.weight)
             bs.append(m.bias)
             bns.append(None)
+            drops.append(0.0)
+            norms.append(norm)
+            if norm is not None and tuple(norm.normalized_shape) != (m.in_features,):
+                raise CardError(f"f_phi: RMSNorm over {tuple(norm.normalized_shape)} ahead of a Linear layer of {m.in_features} inputs")
+            norm, active = None, False
         elif isinstance(m, nn.BatchNorm1d):
             if m.training or not m.track_running_stats:
                 raise CardError("f_phi BatchNorm1d must be in eval mode with running statistics (the reference calls "
                                 "cond_pred_model.eval() before testing, regression/card_regression.py:951)")
-            if not Ws or bns[-1] is not None:
+            if not Ws or bns[-1] is not None or norm is not None:
                 raise CardError("f_phi: BatchNorm1d must follow a Linear layer")
             bns[-1] = m
+            simple = simple and drops[-1] == 0
+        elif norm is not None and isinstance(m, (nn.LeakyReLU, nn.ReLU)):
+            raise CardError("f_phi: an activation between RMSNorm and its Linear layer")
         elif isinstance(m, nn.LeakyReLU):
+            active = True
             if slope is not None and slope != m.negative_slope:
                 raise CardError("f_phi: LeakyReLU layers with different slopes")
             slope = m.negative_slope
         elif isinstance(m, nn.ReLU):
             if slope not in (None, 0.0):
                 raise CardError("f_phi: mixed activation slopes")
-            slope = 0.0
+            slope, active = 0.0, True
         elif isinstance(m, nn.Dropout):
             if m.training and m.p > 0:
                 raise CardError("f_phi Dropout must be in eval mode (identity); call .eval() on the guidance model")
+            if m.p > 0:
+                if not Ws or drops[-1] > 0 or norm is not None:
+                    simple = False
+                else:
+                    drops[-1] = float(m.p)
+        elif isinstance(m, nn.RMSNorm):
+            if norm is not None or (Ws and not active):
+                raise CardError("f_phi: RMSNorm stands once ahead of a Linear layer, behind the activation of the layer before")
+            norm = m
         elif isinstance(m, nn.Identity):
             pass
         else:
             raise CardError(f"f_phi: layer type {type(m).__name__} is not part of regression/model.py:70-79")
     if not Ws:
         raise CardError("f_phi: no Linear layer found")
+    if norm is not None:
+        raise CardError("f_phi: RMSNorm behind the output layer")
+    simple = simple and drops[-1] == 0
     if bns[-1] is not None:
         raise CardError("f_phi: BatchNorm after the output layer is not part of regression/model.py:70-79")
     dims = [int(Ws[0].shape[1])]
@@ -138,7 +283,8 @@ def describe_guidance(net):
         if W.dim() != 2 or int(W.shape[1]) != dims[-1]:
             raise CardError(f"f_phi layer {l}: weight {tuple(W.shape)} does not take {dims[-1]} inputs")
         dims.append(int(W.shape[0]))
-    return {"dims": dims, "weights": Ws, "biases": bs, "batchnorm": bns, "negative_slope": 0.01 if slope is None else float(slope)}
+    return {"dims": dims, "weights": Ws, "biases": bs, "batchnorm": bns, "negative_slope": 0.01 if slope is None else float(slope),
+            "dropout": drops[:-1] if simple else None, "norms": norms}
 
 
 _gcache = weakref.WeakKeyDictionary()

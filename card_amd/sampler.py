@@ -222,6 +222,13 @@ class Sampler:
                 raise CardError(f"fphi_out must be a contiguous fp32 ({rows}, {self.y_dim}) tensor on {self.device}")
             y0 = self.last_y_0_hat = fphi_out
             mu = self._prep(y_T_mean, self.y_dim, "y_T_mean") if y_T_mean is not None else None
+            if fphi._h is None:          # 4-bit weights: f_phi runs ahead of the sampling kernels
+                if fphi.dim_out != self.y_dim:
+                    raise CardError(f"f_phi has {fphi.dim_out} outputs, the sampler's y_dim is {self.y_dim}")
+                if not plan:
+                    fphi.forward(xx, out=fphi_out)
+                mu, fphi = y0 if mu is None else mu, None
+                xx = self._prep(xx, self.x_dim, "x") if self.cat_x and self.x_dim > 0 else None
         else:
             y0 = self._prep(y_0_hat, self.y_dim, "y_0_hat")
             mu = self._prep(y_T_mean, self.y_dim, "y_T_mean")

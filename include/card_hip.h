@@ -397,6 +397,12 @@ CARD_API int card_linear4_forward(const card_linear4* s, const void* x, int32_t 
 CARD_API int card_linear4_quantize(const float* W, int32_t out_features, int32_t in_features, int32_t group, uint8_t* q, float* scale,
                                    uint8_t* zero, void* stream);
 
+/* card_fphi_forward with its Dropout layers active (Monte-Carlo dropout): out (rows, n_z, dim_out), every row with n_z masks.
+ * p: host array of the dropout rates of the n_layers - 1 hidden layers.  Output o of hidden layer l of chain c = row * n_z + z
+ * is dropped as element (chain_offset + c) * dims[l + 1] + o of card_dropout with draw = l. */
+CARD_API int card_fphi_forward_mc(const card_fphi* f, const float* x, int64_t rows, int32_t n_z, const double* p, uint64_t seed,
+                                  uint64_t chain_offset, float* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -145,3 +145,29 @@ def test_reference_formulas():
     y, _ = ref.linear4(torch.tensor([[3, 15]], dtype=torch.uint8), torch.tensor([[2.0]]), torch.tensor([[5]], dtype=torch.uint8), torch.tensor([1.0]), 32,
                        torch.tensor([[1.0, -1.0]]), gamma=torch.tensor([2.0]), slope=0.5)
     assert float(y) == ((3 - 5) * 2 * 1 + (15 - 5) * 2 * -1 + 1) * 2 * 0.5
+
+
+def test_describe_guidance_finds_dropout_rates_and_norms():
+    from torch import nn
+    from card_amd.guidance import describe_guidance
+    net = nn.Sequential(nn.Linear(4, 8), nn.LeakyReLU(), nn.Dropout(0.2), nn.RMSNorm(8), nn.Linear(8, 6), nn.LeakyReLU(), nn.Linear(6, 1)).eval()
+    d = describe_guidance(net)
+    assert d["dropout"] == [0.2, 0.0] and d["norms"] == [None, net[3], None] and d["dims"] == [4, 8, 6, 1]
+    lin = lambda: nn.Linear(4, 4)  # noqa: E731
+    act = nn.LeakyReLU
+    # eval-mode Dropout anywhere is the identity, as ever; its rates are known where one stands behind each hidden layer
+    for layers in ([nn.Dropout(0.1), lin(), act(), lin()], [lin(), act(), nn.Dropout(0.1), nn.Dropout(0.2), lin()], [lin(), act(), lin(), nn.Dropout(0.3)],
+                   [lin(), nn.Dropout(0.3), nn.BatchNorm1d(4), act(), lin()]):
+        assert describe_guidance(nn.Sequential(*layers).eval())["dropout"] is None
+    for layers in ([lin(), nn.RMSNorm(4), lin()], [nn.RMSNorm(5), lin()], [nn.RMSNorm(4), nn.RMSNorm(4), lin()], [lin(), act(), nn.RMSNorm(4)],
+                   [lin(), act(), nn.RMSNorm(4), act(), lin()], [lin(), act(), nn.RMSNorm(4), nn.BatchNorm1d(4), lin()]):
+        with pytest.raises(CardError):
+            describe_guidance(nn.Sequential(*layers).eval())
+
+
+@pytest.mark.parametrize("change,needle", [(dict(rows=-1), "rows"), (dict(n_z=0), "n_z"), (dict(f=None), "null handle"), (dict(rows=1 << 50, n_z=1 << 20), "63 bits")])
+def test_fphi_forward_mc_refusals(change, needle):
+    a = dict(f=P, rows=1, n_z=1)
+    a.update(change)
+    p = (C.c_double * 1)(0.5)
+    assert _lib.lib().card_fphi_forward_mc(a["f"], P, a["rows"], a["n_z"], p, 1, 0, P, None) == E_INVALID and needle in msg(), msg()
