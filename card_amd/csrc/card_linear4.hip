@@ -137,24 +137,34 @@ template <> struct Row8<CARD_DTYPE_E4M3> {
 };
 template <int X> struct Raw { uint32_t w[Row8<X>::kWords]; };
 
-template <int X, bool TAIL> __device__ __forceinline__ Raw<X> load_x(const typename Row8<X>::elem* p, int left) {
-    typedef typename Row8<X>::elem E;
+template <int X> __device__ __forceinline__ Raw<X> load_x(const typename Row8<X>::elem* p) {
+    typedef uint32_t words __attribute__((ext_vector_type(Row8<X>::kWords)));
+    typedef words loose __attribute__((aligned(sizeof(typename Row8<X>::elem))));
+    const words v = *reinterpret_cast<const loose*>(p);
     Raw<X> r;
-    if constexpr (!TAIL) {
-        typedef uint32_t words __attribute__((ext_vector_type(Row8<X>::kWords)));
-        typedef words loose __attribute__((aligned(sizeof(E))));
-        const words v = *reinterpret_cast<const loose*>(p);
 #pragma unroll
-        for (int i = 0; i < Row8<X>::kWords; ++i) r.w[i] = v[i];
+    for (int i = 0; i < Row8<X>::kWords; ++i) r.w[i] = v[i];
+    return r;
+}
+// columns col ... col + 7 of a row of `in`, zeros behind its end: whole vectors where rows end with one, else element by
+// element.  No load waits for another: all are asked for, at the last one's place where there is none.
+template <int X> __device__ __forceinline__ Raw<X> load_tail(const typename Row8<X>::elem* row, int col, int in) {
+    typedef typename Row8<X>::elem E;
+    constexpr int per = 4 / sizeof(E);
+    Raw<X> r;
+    if (in % 8 == 0) {
+        r = load_x<X>(row + (col < in ? col : in - 8));
+#pragma unroll
+        for (int i = 0; i < Row8<X>::kWords; ++i) r.w[i] = col < in ? r.w[i] : 0u;
     } else {
-        constexpr int per = 4 / sizeof(E);
+        uint32_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = row[col + i < in ? col + i : in - 1];
 #pragma unroll
         for (int i = 0; i < Row8<X>::kWords; ++i) {
-            uint32_t v = 0;
+            r.w[i] = 0;
 #pragma unroll
-            for (int j = 0; j < per; ++j)
-                if (i * per + j < left) v |= (uint32_t)p[i * per + j] << (j * 8 * sizeof(E) % 32);
-            r.w[i] = v;
+            for (int j = 0; j < per; ++j) r.w[i] |= (col + i * per + j < in ? e[i * per + j] : 0u) << (j * 8 * sizeof(E) % 32);
         }
     }
     return r;
@@ -310,7 +320,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void linear4_kernel(const Args a, c
     constexpr int W = Row8<X>::kWords;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
-    const int full = a.in / kBlock, b0 = full * wave / waves, b1 = full * (wave + 1) / waves;
+    const bool tail = a.in % kBlock != 0 && wave == waves - 1;
+    const int b0 = a.blocks * wave / waves, b1 = a.blocks * (wave + 1) / waves - tail;
     const int lrow = lane >> 2, lcol = 8 * (lane & 3), from = 4 * (4 * (lane & 15) + (lane >> 4));
     const typename Row8<X>::elem* xr[MT];
 #pragma unroll
@@ -330,7 +341,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void linear4_kernel(const Args a, c
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) g.x[m][s] = load_x<X, false>(xr[m] + b * kBlock + 32 * s, 8);
+            for (int s = 0; s < 4; ++s) g.x[m][s] = load_x<X>(xr[m] + b * kBlock + 32 * s);
     };
     Out out = {};
     if (threadIdx.x < NT * MT * 256) out.ask<MT>(a, threadIdx.x, tile0, m0);
@@ -372,12 +383,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void linear4_kernel(const Args a, c
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (b + u + U < b1) use(st[u]);
-    if (full < a.blocks && wave == waves - 1) {
-        st[0].w.load(a, at, full);
+    if (tail) {
+        st[0].w.load(a, at, b1);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) st[0].x[m][s] = load_x<X, true>(xr[m] + full * kBlock + 32 * s, a.in - (full * kBlock + 32 * s + lcol));
+            for (int s = 0; s < 4; ++s) st[0].x[m][s] = load_tail<X>(xr[m] - lcol, b1 * kBlock + 32 * s + lcol, a.in);
         use(st[0]);
     }
     finish<MT, NT>(a, acc, join, tile0, m0, out, y);
