@@ -170,6 +170,8 @@ class QuantGuidanceNet(GuidanceNet):
     def forward(self, x, out=None):
         """(rows, dim_out) = f_phi(x)."""
         h = self._rows(x)
+        if out is not None and not (tuple(out.shape) == (h.shape[0], self.dim_out) and out.dtype is torch.float32 and out.device == self.device):
+            raise CardError(f"f_phi: out must be ({h.shape[0]}, {self.dim_out}) float32 on {self.device}, got {tuple(out.shape)} {out.dtype} on {out.device}")
         with torch.no_grad():
             h = torch.cat([self._part(h[i:i + _lib.LINEAR4_MAX_ROWS]) for i in range(0, h.shape[0], _lib.LINEAR4_MAX_ROWS)]) \
                 if h.shape[0] > _lib.LINEAR4_MAX_ROWS else self._part(h)

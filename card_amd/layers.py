@@ -67,7 +67,8 @@ def rms_norm_e4m3(x, weight=None, *, residual=None, eps=1e-6):
 
 
 class QuantLinear:
-    """A Linear layer with 4-bit weights, packed on one GPU; immutable after construction (card_linear4).
+    """A Linear layer with 4-bit weights, packed on one GPU (on the current stream); immutable after construction
+    (card_linear4).  It holds the weights that a captured graph reads: keep it as long as the graph.
 
     w[o, k] = (q[o, k] - zero[o, k // group]) * scale[o, k // group]: q (out, in) uint8 with values 0..15, scale (out,
     ceil(in / group)) float32, zero likewise uint8 (0..15) or None = 8 everywhere, bias (out,) or None; group 32, 64 or 128."""

@@ -362,7 +362,8 @@ CARD_API int card_dropout_backward(const void* g, void* dx, int32_t dtype, int64
 CARD_API int card_rms_norm(const void* x, const void* residual, const void* weight, int32_t dtype, int32_t weight_dtype, int64_t rows,
                            int64_t cols, double eps, void* h, void* y, int32_t y_dtype, float* scale, void* stream);
 /* Gradients from h as the forward call stored it (x where there was no residual): g of y and gh of h (either NULL = zeros)
- * give dx (the gradient of x and of the residual) and, unless NULL, dweight (of the weight's type).  dweight needs
+ * give dx (the gradient of x and of the residual) and, unless NULL, dweight (of the weight's type).  dx is rounded once; rows
+ * of at most 8 vectors of 16 bytes are computed in 64 bits (their terms all but cancel).  dweight needs
  * card_rms_norm_backward_workspace_bytes of scratch, 16-byte aligned; its sum over the rows has a fixed order. */
 CARD_API int card_rms_norm_backward_workspace_bytes(int32_t dtype, int64_t rows, int64_t cols, uint64_t* bytes);
 CARD_API int card_rms_norm_backward(const void* h, const void* weight, const void* g, const void* gh, int32_t dtype,
@@ -389,7 +390,8 @@ CARD_API void card_linear4_destroy(card_linear4* s);
 /* y[m, o] = act(gamma[o] * (x_scale[m] * sum_k w[o, k] x[m, k] + bias[o])), act(v) = v > 0 ? v : slope * v.
  * x (rows, in) of any card_dtype; x_scale (rows) goes with CARD_DTYPE_E4M3 and is NULL otherwise; gamma (out) or NULL = ones
  * (a ConditionalLinear's embed.weight[t], regression/model.py:16-17); slope 1 = no activation; y (rows, out) F32, BF16 or F16.
- * Made for one to some tens of rows; at most CARD_LINEAR4_MAX_ROWS.  The weights' device must be current. */
+ * Made for one to some tens of rows; at most CARD_LINEAR4_MAX_ROWS.  The weights' device must be current.  On the way sums hold
+ * up to 31 times the magnitudes of x over a group: x of 2^115 and more may overflow there. */
 CARD_API int card_linear4_forward(const card_linear4* s, const void* x, int32_t x_dtype, const float* x_scale, int64_t rows,
                                   const float* gamma, float slope, void* y, int32_t y_dtype, void* stream);
 /* The nearest such weights of W (out, in) floats: per group scale = (max - min) / 15 over its values and 0, zero = round(-min /

@@ -490,6 +490,104 @@ def test_serving_layer_in_a_captured_graph_and_on_another_stream():
     x.copy_(base)
 
 
+def test_gradients_where_only_some_inputs_ask_for_one():
+    x, r, w, g = rand(6, 130), rand(6, 130, seed=1), 1 + 0.2 * rand(130, seed=2), rand(6, 130, seed=3)
+    gh = rand(6, 130, seed=4)
+    full = [t.clone().requires_grad_(True) for t in (x, r, w)]
+    want = torch.autograd.grad(card_amd.rms_norm(full[0], full[2], residual=full[1]), full, (g, gh))
+    drop = torch.autograd.grad(card_amd.dropout(full[0], 0.3, seed=1, residual=full[1]), full[:2], g)
+    for asks in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1)):
+        t = [v.clone().requires_grad_(bool(a)) for v, a in zip((x, r, w), asks)]
+        leaves = [v for v, a in zip(t, asks) if a]
+        got = torch.autograd.grad(card_amd.rms_norm(t[0], t[2], residual=t[1]), leaves, (g, gh))
+        assert len(got) == sum(asks) and all(torch.equal(a, b) for a, b in zip(got, [v for v, a in zip(want, asks) if a])), asks
+        if asks[0] or asks[1]:
+            leaves = [v for v, a in zip(t[:2], asks) if a]
+            got = torch.autograd.grad(card_amd.dropout(t[0], 0.3, seed=1, residual=t[1]), leaves, g)
+            assert all(torch.equal(a, b) for a, b in zip(got, [v for v, a in zip(drop, asks) if a])), asks
+    # without a residual the weight is the second input
+    wg = w.clone().requires_grad_(True)
+    dw = torch.autograd.grad(card_amd.rms_norm(x, wg), wg, g)[0]
+    assert_within(dw, ref.rms_norm_backward(x, w, g)[1], (6 + chain(130) + 8) * U32 * ref.rms_norm_backward(x, w, g)[3])
+
+
+def test_one_tensor_as_input_and_residual():
+    x, w, g, gh = rand(5, 77), 1 + 0.2 * rand(77, seed=2), rand(5, 77, seed=3), rand(5, 77, seed=4)
+    a, b, c = x.clone().requires_grad_(True), x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    two = torch.autograd.grad(card_amd.rms_norm(b, w, residual=c), (b, c), (g, gh))
+    assert torch.equal(torch.autograd.grad(card_amd.rms_norm(a, w, residual=a), a, (g, gh))[0], two[0] + two[1])
+    two = torch.autograd.grad(card_amd.dropout(b, 0.4, seed=2, residual=c), (b, c), g)
+    assert torch.equal(torch.autograd.grad(card_amd.dropout(a, 0.4, seed=2, residual=a), a, g)[0], two[0] + two[1])
+    # accumulated into .grad, where the two gradients of a norm are one tensor
+    y, h = card_amd.rms_norm(b, w, residual=c)
+    torch.autograd.backward((y, h), (g, gh))
+    first = b.grad.clone()
+    b.grad.mul_(2)
+    assert torch.equal(c.grad, first)
+
+
+def test_second_order_is_refused():
+    x = rand(3, 40).requires_grad_(True)
+    for y in (card_amd.dropout(x, 0.2, seed=1), card_amd.rms_norm(x)):
+        with pytest.raises(RuntimeError, match="first order"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_training_step_in_a_captured_graph():
+    """norm and dropout, forward and backward, captured together; replays with the program's own work in between."""
+    w = (1 + 0.1 * rand(256, seed=2)).requires_grad_(True)
+    x, r = rand(40, 256, dtype=torch.bfloat16).requires_grad_(True), rand(40, 256, seed=1, dtype=torch.bfloat16).requires_grad_(True)
+    g = rand(40, 256, seed=3, dtype=torch.bfloat16)
+
+    def train():
+        d = card_amd.dropout(x, 0.25, seed=9, residual=r)
+        y, h = card_amd.rms_norm(d, w, residual=r)
+        return torch.autograd.grad((y, h), (x, r, w), (g, g))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            train()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = train()
+        graphs.append((graph, got))
+    for k in range(4):
+        with torch.no_grad():
+            x.mul_(1.5)
+            g.add_(0.25)
+        graphs[k % 2][0].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(graphs[k % 2][1], train())), k
+
+
+def test_calls_from_several_threads():
+    import threading
+    x, w = rand(64, 512), 1 + 0.1 * rand(512, seed=1)
+    lin = card_amd.QuantLinear(*weights(96, 512, 64, True), group=64)
+    want = [card_amd.rms_norm(x, w), card_amd.dropout(x, 0.5, seed=3), lin(x)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = [card_amd.rms_norm(x, w), card_amd.dropout(x, 0.5, seed=3), lin(x)]
+                s.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    bad.append(1)
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_refusals_on_the_device():
     x = rand(4, 64)
     with pytest.raises(CardError, match="dtype"):
