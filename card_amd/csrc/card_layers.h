@@ -92,20 +92,14 @@ __device__ __forceinline__ uint32_t keep_bits(const DropRule& d, unsigned long l
     }
     return d.none ? 0u : m >> s;
 }
-// v[j] = kept ? v[j] * scale : 0, for elements e ... e + N - 1
-template <int N> __device__ __forceinline__ void drop(const DropRule& d, unsigned long long seed, unsigned long long e, int n, float (&v)[N]) {
-    if ((e & 3) == 0 && !d.none) {                   // whole blocks: the words decide as they come
+// v[j] = kept ? v[j] * scale : 0 for the N elements of whole blocks from block b on: the words decide as they come
+template <int N> __device__ __forceinline__ void drop(const DropRule& d, unsigned long long seed, unsigned long long b, float (&v)[N]) {
 #pragma unroll
-        for (int k = 0; k < N / 4; ++k) {
-            uint32_t r[4];
-            drop_words(d, seed, (e >> 2) + k, r);
+    for (int k = 0; k < N / 4; ++k) {
+        uint32_t r[4];
+        drop_words(d, seed, b + k, r);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) v[4 * k + w] = r[w] >= d.threshold ? v[4 * k + w] * d.scale : 0.0f;
-        }
-    } else {
-        const uint32_t m = keep_bits<N>(d, seed, e, n);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = (m >> i) & 1 ? v[i] * d.scale : 0.0f;
+        for (int w = 0; w < 4; ++w) v[4 * k + w] = r[w] >= d.threshold && !d.none ? v[4 * k + w] * d.scale : 0.0f;
     }
 }
 
