@@ -51,7 +51,7 @@ struct Shape {
 // One thread per 16 bytes of the output that begin with a whole block of the generator, wherever that is in memory: every
 // block of four words is made once.  n_z > 1: the thread's first element tells row and column, and only where a row ends
 // within the thread's elements are they taken one by one.
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(const Shape s, const DropRule d, const T* x, const T* residual, T* out) {
     constexpr int N = 16 / sizeof(T);
     const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(const Shape s, const 
     const bool whole = from == 0 && n == N;
     if (s.n_z == 1) {
         if (whole) {
-            load_n<N>(x + at, N, v);
+            load_n<N, STREAM>(x + at, N, v);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = i >= from && i < n ? (float)x[at + i] : 0.0f;
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(const Shape s, const 
     }
     if (residual) {
         if (whole) {
-            load_n<N>(residual + at, N, r);
+            load_n<N, STREAM>(residual + at, N, r);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) r[i] = i >= from && i < n ? (float)residual[at + i] : 0.0f;
@@ -168,10 +168,12 @@ int shape_of(const char* who, int32_t dtype, int64_t rows, int64_t cols, int32_t
 
 template <typename T> int forward(const Shape& s, const DropRule& d, const void* x, const void* residual, void* out, hipStream_t stream) {
     constexpr int N = 16 / sizeof(T);
+    const bool past = (s.total * (residual ? 2 : 1) + s.rows * s.cols) * (long long)sizeof(T) > kStreamBytes;
     // as many vectors as the output has, and one more where the first one begins ahead of it
     const long long vectors = s.total / N + 2;
     const unsigned grid = (unsigned)((vectors + kThreads - 1) / kThreads);
-    dropout_kernel<T><<<grid, kThreads, 0, stream>>>(s, d, (const T*)x, (const T*)residual, (T*)out);
+    if (past) dropout_kernel<T, true><<<grid, kThreads, 0, stream>>>(s, d, (const T*)x, (const T*)residual, (T*)out);
+    else dropout_kernel<T, false><<<grid, kThreads, 0, stream>>>(s, d, (const T*)x, (const T*)residual, (T*)out);
     HIP_TRY(hipGetLastError());
     return CARD_OK;
 }

@@ -32,6 +32,7 @@ struct NormArgs {
     long long rows;
     int cols;
     int w_f32;                  // w holds floats whatever x holds
+    bool stream;                // x, residual, g and gh are read past the caches
     float eps;
     // backward
     const void* g;              // NULL: zeros
@@ -96,7 +97,7 @@ template <int L, int K> __device__ __forceinline__ void clear_buf(float (&buf)[K
 }
 
 // a thread's vectors of one row as they lie in memory
-template <typename T, int V> struct RowRaw {
+template <typename T, int V, bool STREAM> struct RowRaw {
     typename Vec<T, 16 / sizeof(T)>::type v[V];
     __device__ __forceinline__ void load(const T* row, int cols, int t, int threads, bool live) {
         constexpr int N = 16 / sizeof(T);
@@ -104,7 +105,7 @@ template <typename T, int V> struct RowRaw {
         for (int k = 0; k < V; ++k) {
             const int c = (k * threads + t) * N, n = live ? cols - c : 0;
             if (n >= N) {
-                v[k] = *reinterpret_cast<const typename Vec<T, N>::loose*>(row + c);
+                v[k] = load_vec<STREAM, N>(row + c);
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) v[k][i] = i < n ? row[c + i] : (T)0.0f;
@@ -131,7 +132,7 @@ __device__ __forceinline__ int pack_e4m3(float a, float b, float c, float d) {
 }
 
 // L lanes per row (0: the workgroup), V vectors per thread
-template <typename T, int L, int V, bool Q>
+template <typename T, int L, int V, bool Q, bool STREAM>
 __global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_kernel(const NormArgs a) {
     constexpr int N = 16 / sizeof(T);
     constexpr bool kAhead = V <= 2;                       // longer rows fill the registers by themselves
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_kernel(const Nor
 #pragma unroll
         for (int v = 0; v < V; ++v) load_w<N, T>(a, (v * threads + t) * N, a.cols - (v * threads + t) * N, w[v]);
     }
-    RowRaw<T, V> x, r;
+    RowRaw<T, V, STREAM> x, r;
     auto fetch = [&](long long at) {
         x.load((const T*)a.x + at * a.cols, a.cols, t, threads, at < a.rows);
         if (a.residual) r.load((const T*)a.residual + at * a.cols, a.cols, t, threads, at < a.rows);
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_kernel(const Nor
 // Six waves to a SIMD (80 registers) are worth more than the last registers: 40000 x 1000 bf16 71 us against 89.
 // F: in rows of a few columns the two terms of dx all but cancel (at one column to eps * rstd^2 of either), so there the
 // row's numbers and the difference are formed in 64 bits.
-template <typename T, typename F, int L, int V>
+template <typename T, typename F, int L, int V, bool STREAM>
 __global__ __launch_bounds__(L ? kThreads : 1024, V == 1 && sizeof(F) == 4 ? 6 : 4) void rms_norm_backward_kernel(const NormArgs a) {
     constexpr int N = 16 / sizeof(T), RPW = L ? kThreads / L : 1;
     static_assert(V <= 2, "longer rows: rms_norm_backward_long_kernel");
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(L ? kThreads : 1024, V == 1 && sizeof(F) == 4 ? 6 :
     float w[V][N], dw[V][N] = {};
 #pragma unroll
     for (int v = 0; v < V; ++v) load_w<N, T>(a, (v * threads + t) * N, a.cols - (v * threads + t) * N, w[v]);
-    RowRaw<T, V> rh, rg, rgh;
+    RowRaw<T, V, STREAM> rh, rg, rgh;
     auto fetch = [&](long long at) {
         rh.load((const T*)a.x + at * a.cols, a.cols, t, threads, at < a.rows);
         rg.load((const T*)a.g + at * a.cols, a.cols, t, threads, a.g && at < a.rows);
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(L ? kThreads : 1024, V == 1 && sizeof(F) == 4 ? 6 :
     if (row < last) fetch(row);
     for (int turn = 0; row < last; row += step, turn ^= 1) {
         const bool live = row < a.rows;
-        const RowRaw<T, V> h = rh, g = rg, gh = rgh;
+        const RowRaw<T, V, STREAM> h = rh, g = rg, gh = rgh;
         F ss = 0, sg = 0;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -430,11 +431,13 @@ template <typename T, bool Q> int forward(const NormArgs& a, hipStream_t st) {
     constexpr int N = 16 / sizeof(T);
     const Form f = form_of(a.cols, N);
     const unsigned grid = (unsigned)groups(f, a.rows, kForwardWaves);
-#define CARD_NORM_CASE(L, V) \
-    if (f.lanes == L && f.v == V) rms_norm_kernel<T, L, V, Q><<<grid, f.threads, 0, st>>>(a)
-    CARD_NORM_CASE(8, 1); CARD_NORM_CASE(16, 1); CARD_NORM_CASE(32, 1); CARD_NORM_CASE(64, 1);
-    CARD_NORM_CASE(0, 1); CARD_NORM_CASE(0, 2); CARD_NORM_CASE(0, 4); CARD_NORM_CASE(0, 8);
-    if constexpr (sizeof(T) == 4) CARD_NORM_CASE(0, 16);
+#define CARD_NORM_CASE(L, V, STREAM) \
+    if (f.lanes == L && f.v == V && (V > 2 || a.stream == STREAM)) rms_norm_kernel<T, L, V, Q, STREAM><<<grid, f.threads, 0, st>>>(a)
+#define CARD_NORM_BOTH(L, V) CARD_NORM_CASE(L, V, false); CARD_NORM_CASE(L, V, true)
+    CARD_NORM_BOTH(8, 1); CARD_NORM_BOTH(16, 1); CARD_NORM_BOTH(32, 1); CARD_NORM_BOTH(64, 1); CARD_NORM_BOTH(0, 1); CARD_NORM_BOTH(0, 2);
+    CARD_NORM_CASE(0, 4, false); CARD_NORM_CASE(0, 8, false);
+    if constexpr (sizeof(T) == 4) CARD_NORM_CASE(0, 16, false);
+#undef CARD_NORM_BOTH
 #undef CARD_NORM_CASE
     HIP_TRY(hipGetLastError());
     return CARD_OK;
@@ -444,10 +447,12 @@ template <typename T> int backward(const NormArgs& a, hipStream_t st) {
     constexpr int N = 16 / sizeof(T);
     const Form f = form_of(a.cols, N);
     const unsigned grid = (unsigned)backward_groups(sizeof(T) == 4 ? CARD_DTYPE_F32 : CARD_DTYPE_BF16, a.rows, a.cols);
-#define CARD_NORM_CASE(F, L, V) \
-    if (f.lanes == L && f.v == V) rms_norm_backward_kernel<T, F, L, V><<<grid, f.threads, 0, st>>>(a)
-    CARD_NORM_CASE(double, 8, 1); CARD_NORM_CASE(float, 16, 1); CARD_NORM_CASE(float, 32, 1); CARD_NORM_CASE(float, 64, 1);
-    CARD_NORM_CASE(float, 0, 1); CARD_NORM_CASE(float, 0, 2);
+#define CARD_NORM_CASE(F, L, V, STREAM) \
+    if (f.lanes == L && f.v == V && a.stream == STREAM) rms_norm_backward_kernel<T, F, L, V, STREAM><<<grid, f.threads, 0, st>>>(a)
+#define CARD_NORM_BOTH(F, L, V) CARD_NORM_CASE(F, L, V, false); CARD_NORM_CASE(F, L, V, true)
+    CARD_NORM_BOTH(double, 8, 1); CARD_NORM_BOTH(float, 16, 1); CARD_NORM_BOTH(float, 32, 1); CARD_NORM_BOTH(float, 64, 1);
+    CARD_NORM_BOTH(float, 0, 1); CARD_NORM_BOTH(float, 0, 2);
+#undef CARD_NORM_BOTH
     if (f.v > 2) rms_norm_backward_long_kernel<T><<<grid, 1024, 0, st>>>(a);
 #undef CARD_NORM_CASE
     HIP_TRY(hipGetLastError());
@@ -461,7 +466,7 @@ int check(const char* who, int32_t dtype, int32_t w_dtype, int64_t rows, int64_t
         return card_fail(CARD_E_INVALID, "%s: weight dtype %d is neither CARD_DTYPE_F32 nor the rows' type %d", who, w_dtype, dtype);
     if (rows < 0 || cols < 1) return card_fail(CARD_E_INVALID, "%s: rows=%lld < 0 or cols=%lld < 1", who, (long long)rows, (long long)cols);
     if (cols > kMaxCols) return card_fail(CARD_E_UNSUPPORTED, "%s: cols=%lld > %d", who, (long long)cols, kMaxCols);
-    if (rows > INT64_MAX / 8 / cols) return card_fail(CARD_E_INVALID, "%s: more bytes than 63 bits count", who);
+    if (rows > INT64_MAX / 16 / cols) return card_fail(CARD_E_INVALID, "%s: more bytes than 63 bits count", who);
     if (!(eps >= 0.0) || isinf(eps)) return card_fail(CARD_E_INVALID, "%s: eps=%g is not a finite number >= 0", who, eps);
     return CARD_OK;
 }
@@ -483,6 +488,8 @@ extern "C" CARD_API int card_rms_norm(const void* x, const void* residual, const
     memset(&a, 0, sizeof(a));
     a.x = x; a.residual = residual; a.w = weight; a.h = h; a.y = y; a.scale = scale;
     a.rows = rows; a.cols = (int)cols; a.w_f32 = weight_dtype == CARD_DTYPE_F32; a.eps = (float)eps;
+    const int64_t eb = card_dtype_bytes(dtype);
+    a.stream = rows * cols * (eb * (residual ? 3 : 1) + (scale ? 1 : eb)) > kStreamBytes;
     hipStream_t st = (hipStream_t)stream;
     if (scale) return dtype == CARD_DTYPE_F32 ? forward<float, true>(a, st) : dtype == CARD_DTYPE_BF16 ? forward<bf16_t, true>(a, st) : forward<f16_t, true>(a, st);
     return dtype == CARD_DTYPE_F32 ? forward<float, false>(a, st) : dtype == CARD_DTYPE_BF16 ? forward<bf16_t, false>(a, st) : forward<f16_t, false>(a, st);
@@ -514,6 +521,7 @@ extern "C" CARD_API int card_rms_norm_backward(const void* h, const void* weight
         NormArgs a;
         memset(&a, 0, sizeof(a));
         a.x = h; a.w = weight; a.y = dx; a.g = g; a.gh = gh; a.rows = rows; a.cols = (int)cols;
+        a.stream = rows * cols * card_dtype_bytes(dtype) * (2 + (g != nullptr) + (gh != nullptr)) > kStreamBytes;
         a.w_f32 = weight_dtype == CARD_DTYPE_F32; a.eps = (float)eps; a.part = dweight ? (float*)workspace : nullptr;
         const int e = dtype == CARD_DTYPE_F32 ? backward<float>(a, st) : dtype == CARD_DTYPE_BF16 ? backward<bf16_t>(a, st) : backward<f16_t>(a, st);
         if (e != CARD_OK) return e;
