@@ -22,7 +22,7 @@ struct card_linear4 {
 
 namespace {
 
-constexpr int kThreads = 256, kBlock = 128, kMaxWaves = 8;
+constexpr int kThreads = 256, kBlock = 128;
 
 // Weights in the order in which the matrix instruction takes them.  Of a tile of 16 outputs and a block of 128 columns lane l
 // holds 16 bytes: word s has the eight values of output l % 16 at the columns 32 s + 8 (l / 16) ... + 7 of the block.  The
@@ -314,8 +314,8 @@ __device__ __forceinline__ void finish(const Args& a, const f32x4 (&acc)[MT][NT]
 // asks for row l / 4 -- four lanes share a row's 64 bytes -- and ds_bpermute hands the values over where they are used; LDS
 // between them took as long and needs barriers.  U blocks of weights and of x are on their way while one is used: the loop
 // over them has no branch, or every wait in it would be for all of them.  A last block that is not full comes after the loop.
-template <int X, int G, int MT, int NT, int U, bool STREAM>
-__global__ __launch_bounds__(64 * kMaxWaves) void linear4_kernel(const Args a, const typename Row8<X>::elem* x, void* y) {
+template <int X, int G, int MT, int NT, int U, bool STREAM, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Args a, const typename Row8<X>::elem* x, void* y) {
     extern __shared__ float join[];                  // (waves, NT, MT, 4, 64)
     constexpr int W = Row8<X>::kWords;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -394,26 +394,26 @@ __global__ __launch_bounds__(64 * kMaxWaves) void linear4_kernel(const Args a, c
     finish<MT, NT>(a, acc, join, tile0, m0, out, y);
 }
 
-template <int X, int G, int MT, int NT, int U, bool STREAM> int launch(const Args& a, const void* x, void* y, hipStream_t st) {
+template <int X, int G, int MT, int NT, int U, bool STREAM, int WAVES> int launch(const Args& a, const void* x, void* y, hipStream_t st) {
     int waves = 1;                                   // a block of columns for each at least
-    while (waves < kMaxWaves && a.blocks >= 2 * waves) waves *= 2;
+    while (waves < WAVES && a.blocks >= 2 * waves) waves *= 2;
     const dim3 grid((a.tiles + NT - 1) / NT, (a.rows + 16 * MT - 1) / (16 * MT));
-    linear4_kernel<X, G, MT, NT, U, STREAM><<<grid, 64 * waves, waves * NT * MT * 256 * sizeof(float), st>>>(a, (const typename Row8<X>::elem*)x, y);
+    linear4_kernel<X, G, MT, NT, U, STREAM, WAVES><<<grid, 64 * waves, waves * NT * MT * 256 * sizeof(float), st>>>(a, (const typename Row8<X>::elem*)x, y);
     HIP_TRY(hipGetLastError());
     return CARD_OK;
 }
 // Several tiles share the values of x where there are more tiles than CUs (24 rows, 6144 outputs: 9.8 us with two against
 // 10.3).  From 1024 tiles on the weights pass by the caches, which cannot hold them (16 rows of 8192 columns, 28672 outputs:
-// 29.7 us against 31.5; but 5.8 against 5.1 for 4096 x 4096, whose weights stay in L2 from call to call), and there `wide`
-// rows -- more than 16, or fp32 with its three operands -- take four tiles and one block on its way in the registers that
-// hold two and two otherwise (8192 columns, 28672 outputs: 32 rows bf16 44 us against 50, 16 rows fp32 49 against 71; one row
-// bf16 31 against 28).
+// 29.7 us against 31.5; but 5.8 against 5.1 for 4096 x 4096, whose weights stay in L2 from call to call), and workgroups are
+// plenty: four tiles and four waves with one block on its way, so that a CU holds four workgroups (8192 columns, 28672
+// outputs: 16 rows bf16 29.2 us against 34.5 with two tiles, eight waves and two blocks, fp32 45.5 and 48.9, 32 rows e4m3
+// 37.7 and 42.7; 17000 outputs of 4096 columns 14.5 and 13.3).
 constexpr int kCus = 256, kStreamTiles = 1024;
 template <int X, int G, int MT> int by_tiles(const Args& a, const void* x, void* y, hipStream_t st) {
-    constexpr bool wide = X == CARD_DTYPE_F32 || MT > 1;
-    constexpr int U = wide ? 1 : 2;
-    if (a.tiles <= kCus) return launch<X, G, MT, 1, U, false>(a, x, y, st);
-    return a.tiles < kStreamTiles ? launch<X, G, MT, 2, U, false>(a, x, y, st) : launch<X, G, MT, wide ? 4 : 2, U, true>(a, x, y, st);
+    // blocks on their way: one where rows are wide -- more than 16, or fp32 with its three operands -- for the registers' sake
+    constexpr int U = X == CARD_DTYPE_F32 || MT > 1 ? 1 : 2;
+    if (a.tiles <= kCus) return launch<X, G, MT, 1, U, false, 8>(a, x, y, st);
+    return a.tiles < kStreamTiles ? launch<X, G, MT, 2, U, false, 8>(a, x, y, st) : launch<X, G, MT, 4, 1, true, 4>(a, x, y, st);
 }
 template <int X, int G> int by_rows(const Args& a, const void* x, void* y, hipStream_t st) {
     return a.rows <= 16 ? by_tiles<X, G, 1>(a, x, y, st) : by_tiles<X, G, 2>(a, x, y, st);
