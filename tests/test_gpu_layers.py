@@ -347,7 +347,7 @@ def lin_bound(want, size, group, in_f, out_dtype):
 
 
 SHAPES = [(1, 1, 1), (1, 64, 16), (2, 31, 33), (3, 100, 50), (5, 1001, 77), (16, 128, 128), (17, 129, 15), (33, 257, 100), (64, 512, 48), (1, 4096, 512),
-          (8, 2048, 1000), (100, 300, 130)]
+          (8, 2048, 1000), (100, 300, 130), (9, 392, 5000), (3, 200, 16400), (20, 136, 16389), (40, 129, 16384)]
 
 
 @pytest.mark.parametrize("rows,in_f,out_f", SHAPES)
@@ -562,6 +562,33 @@ def test_training_step_in_a_captured_graph():
         graphs[k % 2][0].replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(graphs[k % 2][1], train())), k
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+@pytest.mark.parametrize("cols", [40, 200, 1000, 6001, 9000])
+def test_large_calls_are_their_parts(dtype, cols):
+    """Calls of more than 300 MB take kernels of their own: a row has the same bits there as in a small call."""
+    rows = 320_000_000 // (4 * cols * dtype.itemsize) + 37
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x, r, g, gh = (torch.randn(rows, cols, device=DEV, generator=gen).to(dtype) for _ in range(4))
+    w = 1 + 0.1 * rand(cols, seed=2)
+    part = slice(rows - 50, rows)
+
+    def train(x, r, g, gh, offset):
+        a, b, c = x.clone().requires_grad_(True), r.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        y, h = card_amd.rms_norm(a, c, residual=b)
+        dx = torch.autograd.grad((y, h), (a, c), (g, gh))
+        d = card_amd.dropout(a, 0.3, seed=5, elem_offset=offset, residual=b)
+        q, s, h8 = card_amd.rms_norm_e4m3(x, w, residual=r)
+        return [y, h, dx[0], d, torch.autograd.grad(d, a, g)[0], q.view(torch.uint8), s, h8, card_amd.rms_norm(x, w), card_amd.dropout(x, 0.3, seed=5, elem_offset=offset)], dx[1]
+    whole, dw = train(x, r, g, gh, 0)
+    parts, _ = train(x[part], r[part], g[part], gh[part], (rows - 50) * cols)
+    for k, (a, b) in enumerate(zip(whole, parts)):
+        assert torch.equal(a[part], b), k
+    # the weight's gradient in 64 bits, on the device: rows + chain() + 8 roundings of the sum of magnitudes at most
+    h = whole[1].double()
+    unit = g.double() * h / torch.sqrt((h * h).mean(-1, keepdim=True) + 1e-6)
+    assert bool(((dw.double() - unit.sum(0)).abs() <= (rows + chain(cols) + 8) * U32 * unit.abs().sum(0)).all())
 
 
 def test_calls_from_several_threads():
