@@ -19,7 +19,7 @@ EXPORTS = (
     "card_fphi_create", "card_fphi_destroy", "card_fphi_forward", "card_sampler_plan",
     "card_dropout", "card_dropout_backward", "card_rms_norm", "card_rms_norm_backward",
     "card_rms_norm_backward_workspace_bytes", "card_linear4_create", "card_linear4_destroy", "card_linear4_forward",
-    "card_linear4_quantize", "card_fphi_forward_mc",
+    "card_linear4_quantize", "card_linear4_workspace_bytes", "card_fphi_forward_mc",
 )
 FPHI_MAX_LAYERS, FPHI_MAX_WIDTH = 8, 1024
 NORM_MAX_COLS = 65536
@@ -136,7 +136,8 @@ def lib():
     L.card_linear4_create.argtypes = [C.POINTER(Linear4Desc), C.c_void_p, C.POINTER(C.c_void_p)]
     L.card_linear4_destroy.argtypes = [C.c_void_p]
     L.card_linear4_destroy.restype = None
-    L.card_linear4_forward.argtypes = [C.c_void_p, _fp, i32, _fp, i64, _fp, C.c_float, _fp, i32, C.c_void_p]
+    L.card_linear4_forward.argtypes = [C.c_void_p, _fp, i32, _fp, i64, _fp, C.c_float, _fp, i32, _fp, u64, C.c_void_p]
+    L.card_linear4_workspace_bytes.argtypes = [C.c_void_p, i32, i64, C.POINTER(u64)]
     L.card_fphi_forward_mc.argtypes = [C.c_void_p, _fp, i64, i32, C.POINTER(f64), u64, u64, _fp, C.c_void_p]
     L.card_linear4_quantize.argtypes = [_fp, i32, i32, i32, _fp, _fp, _fp, C.c_void_p]
     for name in EXPORTS:

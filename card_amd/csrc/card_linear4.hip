@@ -85,6 +85,8 @@ struct Args {
     int in, out, blocks, tiles;
     int rows;
     int y_dtype;
+    float* partial;            // (splits, rows, out): sums of a share of the columns each, or NULL: one share
+    int splits;
 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -264,6 +266,16 @@ __device__ __forceinline__ void add_block(const Weights<G, NT, STREAM>& w, uint3
     }
 }
 
+__device__ __forceinline__ float epilogue(const Args& a, float v, float x_scale, float bias, float gamma) {
+    v = (v * x_scale + bias) * gamma;
+    return v > 0.0f ? v : v * a.slope;
+}
+__device__ __forceinline__ void store_y(const Args& a, void* y, long long at, float v) {
+    if (a.y_dtype == CARD_DTYPE_F32) ((float*)y)[at] = v;
+    else if (a.y_dtype == CARD_DTYPE_BF16) ((bf16_t*)y)[at] = (bf16_t)v;
+    else ((f16_t*)y)[at] = (f16_t)v;
+}
+
 // What the epilogue multiplies and adds for one output: asked for at the start, so that it has come by the end.
 struct Out {
     int row;
@@ -298,13 +310,21 @@ __device__ __forceinline__ void finish(const Args& a, const f32x4 (&acc)[MT][NT]
         if (!out.real) continue;
         float v = join[id];
         for (int w = 1; w < waves; ++w) v += join[w * n + id];
-        v = (v * out.x_scale + out.bias) * out.gamma;
-        v = v > 0.0f ? v : v * a.slope;
         const long long at = (long long)out.row * a.out + out.o;
-        if (a.y_dtype == CARD_DTYPE_F32) ((float*)y)[at] = v;
-        else if (a.y_dtype == CARD_DTYPE_BF16) ((bf16_t*)y)[at] = (bf16_t)v;
-        else ((f16_t*)y)[at] = (f16_t)v;
+        if (a.partial) a.partial[(long long)blockIdx.z * a.rows * a.out + at] = v;
+        else store_y(a, y, at, epilogue(a, v, out.x_scale, out.bias, out.gamma));
     }
+}
+
+// the shares of the columns join in a fixed order
+__global__ __launch_bounds__(kThreads) void linear4_join_kernel(const Args a, void* y) {
+    const long long id = (long long)blockIdx.x * kThreads + threadIdx.x, n = (long long)a.rows * a.out;
+    if (id >= n) return;
+    const int row = (int)(id / a.out), o = (int)(id - (long long)row * a.out);
+    float v = a.partial[id];
+#pragma unroll 4
+    for (int k = 1; k < a.splits; ++k) v += a.partial[k * n + id];
+    store_y(a, y, id, epilogue(a, v, a.x_scale ? a.x_scale[row] : 1.0f, a.bias[o], a.gamma ? a.gamma[o] : 1.0f));
 }
 
 // One workgroup: 16 MT rows of x by 16 NT outputs; each of its waves takes a run of blocks of columns.
@@ -320,8 +340,9 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Args a, const
     constexpr int W = Row8<X>::kWords;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int tile0 = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
-    const bool tail = a.in % kBlock != 0 && wave == waves - 1;
-    const int b0 = a.blocks * wave / waves, b1 = a.blocks * (wave + 1) / waves - tail;
+    const int s0 = a.blocks * blockIdx.z / gridDim.z, n = a.blocks * (blockIdx.z + 1) / gridDim.z - s0;          // this share's blocks
+    const bool tail = a.in % kBlock != 0 && wave == waves - 1 && blockIdx.z == gridDim.z - 1;
+    const int b0 = s0 + n * wave / waves, b1 = s0 + n * (wave + 1) / waves - tail;
     const int lrow = lane >> 2, lcol = 8 * (lane & 3), from = 4 * (4 * (lane & 15) + (lane >> 4));
     const typename Row8<X>::elem* xr[MT];
 #pragma unroll
@@ -396,11 +417,27 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Args a, const
 
 template <int X, int G, int MT, int NT, int U, bool STREAM, int WAVES> int launch(const Args& a, const void* x, void* y, hipStream_t st) {
     int waves = 1;                                   // a block of columns for each at least
-    while (waves < WAVES && a.blocks >= 2 * waves) waves *= 2;
-    const dim3 grid((a.tiles + NT - 1) / NT, (a.rows + 16 * MT - 1) / (16 * MT));
+    while (waves < WAVES && a.blocks / a.splits >= 2 * waves) waves *= 2;
+    const dim3 grid((a.tiles + NT - 1) / NT, (a.rows + 16 * MT - 1) / (16 * MT), a.splits);
     linear4_kernel<X, G, MT, NT, U, STREAM, WAVES><<<grid, 64 * waves, waves * NT * MT * 256 * sizeof(float), st>>>(a, (const typename Row8<X>::elem*)x, y);
     HIP_TRY(hipGetLastError());
+    if (a.partial) {
+        linear4_join_kernel<<<(unsigned)(((long long)a.rows * a.out + kThreads - 1) / kThreads), kThreads, 0, st>>>(a, y);
+        HIP_TRY(hipGetLastError());
+    }
     return CARD_OK;
+}
+// Shares of the columns, where there are too few tiles for the chip and a workgroup would be long at its columns: one for every
+// eight blocks (a block for each of its waves) while the chip has CUs for them.  The second launch costs some 3 us, so it has to
+// be long: a wave's blocks, weighted by the row tiles and by fp32's three operands, are 24 or more (12000 columns, 100 outputs:
+// 30 rows fp32 33 us in one share and 13.5 in eleven, 30 rows bf16 12.9 and 9.2; below, 16 rows fp16 8.6 and 8.7, 8000 columns
+// of 30 rows e4m3 8.5 and 9.4).
+int splits_of(int tiles, int blocks, int64_t rows, int x_dtype) {
+    const int row_tiles = rows <= 16 ? 1 : 2, work = (blocks + 7) / 8 * row_tiles * (x_dtype == CARD_DTYPE_F32 ? 3 : 1);
+    const int64_t groups = tiles * ((rows + 16 * row_tiles - 1) / (16 * row_tiles));
+    if (tiles > 128 || work < 24) return 1;
+    const int64_t most = 256 / groups, s = blocks / 8 < most ? blocks / 8 : most;
+    return s > 1 ? (int)s : 1;
 }
 // Several tiles share the values of x where there are more tiles than CUs (24 rows, 6144 outputs: 9.8 us with two against
 // 10.3).  From 1024 tiles on the weights pass by the caches, which cannot hold them (16 rows of 8192 columns, 28672 outputs:
@@ -485,8 +522,20 @@ extern "C" CARD_API void card_linear4_destroy(card_linear4* s) {
     delete s;
 }
 
+extern "C" CARD_API int card_linear4_workspace_bytes(const card_linear4* s, int32_t x_dtype, int64_t rows, uint64_t* bytes) {
+    const char* who = "card_linear4_workspace_bytes";
+    if (!s || !bytes) return card_fail(CARD_E_INVALID, "%s: null argument", who);
+    if (!card_dtype_bytes(x_dtype)) return card_fail(CARD_E_INVALID, "%s: x_dtype %d is no card_dtype", who, x_dtype);
+    if (rows < 0) return card_fail(CARD_E_INVALID, "%s: rows=%lld < 0", who, (long long)rows);
+    if (rows > CARD_LINEAR4_MAX_ROWS) return card_fail(CARD_E_UNSUPPORTED, "%s: rows=%lld > %d", who, (long long)rows, CARD_LINEAR4_MAX_ROWS);
+    const int n = rows ? splits_of(s->tiles, s->blocks, rows, x_dtype) : 1;
+    *bytes = n > 1 ? (uint64_t)n * (uint64_t)rows * (uint64_t)s->out * sizeof(float) : 0;
+    return CARD_OK;
+}
+
 extern "C" CARD_API int card_linear4_forward(const card_linear4* s, const void* x, int32_t x_dtype, const float* x_scale, int64_t rows,
-                                             const float* gamma, float slope, void* y, int32_t y_dtype, void* stream) {
+                                             const float* gamma, float slope, void* y, int32_t y_dtype, void* workspace,
+                                             uint64_t workspace_bytes, void* stream) {
     const char* who = "card_linear4_forward";
     if (!s) return card_fail(CARD_E_INVALID, "%s: null handle", who);
     if (!card_dtype_bytes(x_dtype)) return card_fail(CARD_E_INVALID, "%s: x_dtype %d is no card_dtype", who, x_dtype);
@@ -504,6 +553,14 @@ extern "C" CARD_API int card_linear4_forward(const card_linear4* s, const void* 
     Args a;
     a.q = s->q; a.scale = s->scale; a.zero = s->zero; a.bias = s->bias; a.x_scale = x_scale; a.gamma = gamma; a.slope = slope;
     a.in = s->in; a.out = s->out; a.blocks = s->blocks; a.tiles = s->tiles; a.rows = (int)rows; a.y_dtype = y_dtype;
+    a.splits = splits_of(s->tiles, s->blocks, rows, x_dtype);
+    a.partial = a.splits > 1 ? (float*)workspace : nullptr;
+    if (a.splits > 1) {
+        const uint64_t need = (uint64_t)a.splits * (uint64_t)rows * (uint64_t)s->out * sizeof(float);
+        if (!workspace || workspace_bytes < need)
+            return card_fail(CARD_E_INVALID, "%s: workspace of %llu bytes, need %llu", who, (unsigned long long)workspace_bytes, (unsigned long long)need);
+        if ((uintptr_t)workspace & 15) return card_fail(CARD_E_INVALID, "%s: workspace is not 16-byte aligned", who);
+    }
     hipStream_t st = (hipStream_t)stream;
     switch (x_dtype) {
         case CARD_DTYPE_F32: return by_group<CARD_DTYPE_F32>(a, s->group, x, y, st);

@@ -29,6 +29,7 @@ struct {
     decltype(&card_rms_norm_backward) rms_norm_backward;
     decltype(&card_rms_norm_backward_workspace_bytes) rms_norm_backward_workspace_bytes;
     decltype(&card_linear4_forward) linear4_forward;
+    decltype(&card_linear4_workspace_bytes) linear4_workspace_bytes;
 } lib;
 PyObject* card_error;
 
@@ -248,15 +249,18 @@ Tensor linear4(uintptr_t handle, int64_t device, int64_t in, int64_t out, const 
     auto shape = x.sizes().vec();
     shape.back() = out;
     Tensor y = at::empty(shape, x.options().dtype(ot));
+    uint64_t bytes = 0;
+    check(lib.linear4_workspace_bytes((const card_linear4*)handle, xt, xc.numel() / in, &bytes), "card_linear4_forward");
+    const Tensor ws = bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : Tensor();
     check(lib.linear4_forward((const card_linear4*)handle, ptr(xc), xt, (const float*)ptr(x_scale), xc.numel() / in, (const float*)ptr(gamma), (float)slope, ptr(y),
-                              ot == at::kFloat ? CARD_DTYPE_F32 : ot == at::kBFloat16 ? CARD_DTYPE_BF16 : CARD_DTYPE_F16, stream_of(x)), "card_linear4_forward");
+                              ot == at::kFloat ? CARD_DTYPE_F32 : ot == at::kBFloat16 ? CARD_DTYPE_BF16 : CARD_DTYPE_F16, ptr(ws), bytes, stream_of(x)), "card_linear4_forward");
     return y;
 }
 
 void init(py::dict address, py::object error) {
 #define CARD_TAKE(name) lib.name = reinterpret_cast<decltype(lib.name)>(address["card_" #name].cast<uintptr_t>())
     CARD_TAKE(last_error); CARD_TAKE(dropout); CARD_TAKE(dropout_backward); CARD_TAKE(rms_norm); CARD_TAKE(rms_norm_backward);
-    CARD_TAKE(rms_norm_backward_workspace_bytes); CARD_TAKE(linear4_forward);
+    CARD_TAKE(rms_norm_backward_workspace_bytes); CARD_TAKE(linear4_forward); CARD_TAKE(linear4_workspace_bytes);
 #undef CARD_TAKE
     card_error = error.inc_ref().ptr();
 }

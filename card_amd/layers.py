@@ -30,7 +30,7 @@ def _load():
             raise CardError(f"{_EXT_PATH} is missing: build it with `make -C card_amd/csrc` (or __graft_entry__.build()).")
         from . import _card_torch
         names = ("card_last_error", "card_dropout", "card_dropout_backward", "card_rms_norm", "card_rms_norm_backward",
-                 "card_rms_norm_backward_workspace_bytes", "card_linear4_forward")
+                 "card_rms_norm_backward_workspace_bytes", "card_linear4_forward", "card_linear4_workspace_bytes")
         _card_torch.init({n: C.cast(getattr(L, n), C.c_void_p).value for n in names}, CardError)
         _ext = _card_torch
     return _ext

@@ -391,9 +391,13 @@ CARD_API void card_linear4_destroy(card_linear4* s);
  * x (rows, in) of any card_dtype; x_scale (rows) goes with CARD_DTYPE_E4M3 and is NULL otherwise; gamma (out) or NULL = ones
  * (a ConditionalLinear's embed.weight[t], regression/model.py:16-17); slope 1 = no activation; y (rows, out) F32, BF16 or F16.
  * Made for one to some tens of rows; at most CARD_LINEAR4_MAX_ROWS.  The weights' device must be current.  On the way sums hold
- * up to 31 times the magnitudes of x over a group: x of 2^115 and more may overflow there. */
+ * up to 31 times the magnitudes of x over a group: x of 2^115 and more may overflow there.
+ * workspace: card_linear4_workspace_bytes of scratch (0 for most shapes; then NULL is fine), 16-byte aligned; calls that share
+ * one must not overlap in time. */
+CARD_API int card_linear4_workspace_bytes(const card_linear4* s, int32_t x_dtype, int64_t rows, uint64_t* bytes);
 CARD_API int card_linear4_forward(const card_linear4* s, const void* x, int32_t x_dtype, const float* x_scale, int64_t rows,
-                                  const float* gamma, float slope, void* y, int32_t y_dtype, void* stream);
+                                  const float* gamma, float slope, void* y, int32_t y_dtype, void* workspace, uint64_t workspace_bytes,
+                                  void* stream);
 /* The nearest such weights of W (out, in) floats: per group scale = (max - min) / 15 over its values and 0, zero = round(-min /
  * scale), q = round(w / scale) + zero.  q (out, in), scale and zero (out, ceil(in / group)). */
 CARD_API int card_linear4_quantize(const float* W, int32_t out_features, int32_t in_features, int32_t group, uint8_t* q, float* scale,

@@ -347,7 +347,8 @@ def lin_bound(want, size, group, in_f, out_dtype):
 
 
 SHAPES = [(1, 1, 1), (1, 64, 16), (2, 31, 33), (3, 100, 50), (5, 1001, 77), (16, 128, 128), (17, 129, 15), (33, 257, 100), (64, 512, 48), (1, 4096, 512),
-          (8, 2048, 1000), (100, 300, 130), (9, 392, 5000), (3, 200, 16400), (20, 136, 16389), (40, 129, 16384)]
+          (8, 2048, 1000), (100, 300, 130), (9, 392, 5000), (3, 200, 16400), (20, 136, 16389), (40, 129, 16384),
+          (30, 4100, 40), (20, 12300, 24), (40, 4216, 33), (3, 9000, 17)]
 
 
 @pytest.mark.parametrize("rows,in_f,out_f", SHAPES)
@@ -383,6 +384,29 @@ def test_linear4_row_results_do_not_depend_on_their_neighbours():
     y = lin.forward(bad)
     keep = [i for i in range(64) if i not in (5, 40)]
     assert torch.equal(y[keep], clean[keep]) and bool(torch.isnan(y[5]).all()) and not bool(torch.isfinite(y[40]).any())
+
+
+def test_linear4_shares_of_the_columns_need_their_workspace():
+    """Few outputs and long rows: the columns are split over workgroups, with the caller's scratch between the two launches."""
+    import ctypes as C
+    from card_amd import _lib
+    L = _lib.lib()
+    q, s, z, b = weights(40, 4100, 128, True)
+    lin = card_amd.QuantLinear(q, s, z, b, group=128)
+    x, y, n = rand(30, 4100), torch.full((30, 40), 7.0, device=DEV), C.c_uint64()
+    assert L.card_linear4_workspace_bytes(lin._h, _lib.DTYPE_F32, 30, C.byref(n)) == 0 and n.value >= 2 * 30 * 40 * 4
+    ws = torch.empty(n.value + 8, dtype=torch.uint8, device=DEV)
+    call = lambda w, k: L.card_linear4_forward(lin._h, x.data_ptr(), _lib.DTYPE_F32, None, 30, None, 1.0, y.data_ptr(), _lib.DTYPE_F32, w, k, None)  # noqa: E731
+    for w, k in ((None, 0), (None, n.value), (ws.data_ptr(), n.value - 1), (ws.data_ptr() + 8, n.value)):
+        assert call(w, k) == -1 and "workspace" in L.card_last_error().decode()
+    torch.cuda.synchronize()
+    assert bool((y == 7).all())
+    assert call(ws.data_ptr(), n.value) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y, lin(x))
+    assert L.card_linear4_workspace_bytes(lin._h, _lib.DTYPE_BF16, 1, C.byref(n)) == 0 and n.value == 0
+    assert L.card_linear4_workspace_bytes(lin._h, 9, 1, C.byref(n)) == -1 and L.card_linear4_workspace_bytes(lin._h, 0, -1, C.byref(n)) == -1
+    assert L.card_linear4_workspace_bytes(lin._h, 0, 65536, C.byref(n)) == -2
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)

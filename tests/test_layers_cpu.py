@@ -88,10 +88,12 @@ def test_linear4_other_refusals():
     L = _lib.lib()
     h = C.c_void_p()
     assert L.card_linear4_create(None, None, C.byref(h)) == E_INVALID
-    assert L.card_linear4_forward(None, P, 0, None, 1, None, 1.0, P, 0, None) == E_INVALID and "null handle" in msg()
+    assert L.card_linear4_forward(None, P, 0, None, 1, None, 1.0, P, 0, None, 0, None) == E_INVALID and "null handle" in msg()
     assert L.card_linear4_quantize(P, 4, 4, 48, P, P, P, None) == E_UNSUPPORTED
     assert L.card_linear4_quantize(P, 0, 4, 32, P, P, P, None) == E_INVALID
     assert L.card_linear4_quantize(None, 4, 4, 32, P, P, P, None) == E_INVALID
+    n = C.c_uint64()
+    assert L.card_linear4_workspace_bytes(None, 0, 1, C.byref(n)) == E_INVALID and "null" in msg()
     L.card_linear4_destroy(None)
 
 
