@@ -11,8 +11,8 @@
 // What bounds it is memory: a row is read once and lives in registers, V vectors of 16 bytes in each thread of a workgroup
 // of as many waves as the row needs (up to 64 vectors: 8, 16, 32 or 64 lanes).  A workgroup walks over rows with the weight in
 // registers and asks for the next row before it joins the sums of this one, so loads are on their way all the time.
-// 8192 x 6144 bf16 with residual: forward 63 us (6.4 TB/s), backward 92 us (4.4 TB/s) and 4 us to join dw; 8192 x 4096 to e4m3
-// 44 us (5.3 TB/s); one row of 4096 2.6 us.  A large copy reaches 5.5 TB/s on this card.
+// 8192 x 6144 bf16 with residual: forward 60 us (6.7 TB/s), backward 68 us (6.0 TB/s) and 4 us to join dw; 8192 x 4096 to e4m3
+// 44 us back to back (5.3 TB/s); one row of 4096 2.5 us.  A large copy reaches 5.5 TB/s on this card.
 #include "card_layers.h"
 
 using namespace card;
