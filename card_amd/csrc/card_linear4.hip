@@ -443,14 +443,17 @@ int splits_of(int tiles, int blocks, int64_t rows, int x_dtype) {
 // 10.3).  From 1024 tiles on the weights pass by the caches, which cannot hold them (16 rows of 8192 columns, 28672 outputs:
 // 29.7 us against 31.5; but 5.8 against 5.1 for 4096 x 4096, whose weights stay in L2 from call to call), and workgroups are
 // plenty: four tiles and four waves with one block on its way, so that a CU holds four workgroups (8192 columns, 28672
-// outputs: 16 rows bf16 29.2 us against 34.5 with two tiles, eight waves and two blocks, fp32 45.5 and 48.9, 32 rows e4m3
-// 37.7 and 42.7; 17000 outputs of 4096 columns 14.5 and 13.3).
+// outputs: 16 rows bf16 30.2 us against 34.8 with two tiles, eight waves and two blocks, fp32 45.3 and 68.0, 32 rows e4m3
+// 40.0 and 51.1).  Up to 16 rows of e4m3, half of bf16's x to read, need only three tiles to share them, and smaller workgroups
+// even out the last ones (28672 outputs 29.4 us against 29.9 with four, 17000 outputs of 4096 columns 12.2 and 14.5; but bf16
+// 33.0 against 30.2).
 constexpr int kCus = 256, kStreamTiles = 1024;
 template <int X, int G, int MT> int by_tiles(const Args& a, const void* x, void* y, hipStream_t st) {
     // blocks on their way: one where rows are wide -- more than 16, or fp32 with its three operands -- for the registers' sake
     constexpr int U = X == CARD_DTYPE_F32 || MT > 1 ? 1 : 2;
     if (a.tiles <= kCus) return launch<X, G, MT, 1, U, false, 8>(a, x, y, st);
-    return a.tiles < kStreamTiles ? launch<X, G, MT, 2, U, false, 8>(a, x, y, st) : launch<X, G, MT, 4, 1, true, 4>(a, x, y, st);
+    if (a.tiles < kStreamTiles) return launch<X, G, MT, 2, U, false, 8>(a, x, y, st);
+    return launch<X, G, MT, X == CARD_DTYPE_E4M3 && MT == 1 ? 3 : 4, 1, true, 4>(a, x, y, st);
 }
 template <int X, int G> int by_rows(const Args& a, const void* x, void* y, hipStream_t st) {
     return a.rows <= 16 ? by_tiles<X, G, 1>(a, x, y, st) : by_tiles<X, G, 2>(a, x, y, st);
