@@ -49,16 +49,37 @@ void on_gpu(const Tensor& t) {
     if (!t.is_cuda())
         refuse("card_amd runs on an AMD GPU only (the tensor is on '", t.device().str(), "'); there is no CPU fallback. Move the model and inputs to cuda.");
 }
-Tensor same(const Tensor& t, const Tensor& like, at::IntArrayRef shape, const char* name) {
+void same(const Tensor& t, const Tensor& like, at::IntArrayRef shape, const char* name) {
     if (t.sizes() != shape || t.scalar_type() != like.scalar_type() || t.device() != like.device())
         refuse(name, ": expected ", shape, " ", like.scalar_type(), " on ", like.device().str(), ", got ", t.sizes(), " ", t.scalar_type(), " on ", t.device().str());
-    return t.contiguous();
 }
+Tensor dense(const OptTensor& t) { return t ? t->contiguous() : Tensor(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
-void first_order(const char* what) {
+bool capturing(const c10::hip::HIPStream& s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(s.stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+}
+// What a backward pass is refused for.  A leaf's gradient node remembers the stream it was made on, and lives as long as any
+// graph of the leaf.  Into a capture that began after it, the engine would draw that stream with a wait that is not allowed
+// there, and the process would not survive the capture's end.
+void check_backward(const char* what) {
     if (at::GradMode::is_enabled()) refuse(what, ": the backward pass is of first order only (create_graph=True asks for more)");
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    const auto current = c10::hip::getCurrentHIPStream();
+    if (!capturing(current)) return;
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+        const auto& next = node->next_edge(i).function;
+        if (!next || !node->task_should_compute_output(i)) continue;
+        const auto stream = next->stream();
+        if (!stream || (stream->id() == current.id() && stream->device_index() == current.device_index())) continue;
+        const c10::hip::HIPStream other(c10::hip::HIPStream::UNCHECKED, c10::Stream(c10::Stream::UNSAFE, current.device(), stream->id()));
+        if (stream->id() == 0 || !capturing(other))          // 0: the default stream, which is never captured
+            refuse(what, ": this backward pass is being captured, but an input's gradient belongs to another stream: a graph of the same "
+                   "tensors from before the capture is still alive. Drop its results first, or make them on the capture's stream");
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ dropout
@@ -85,6 +106,7 @@ Tensor drop_forward(const Tensor& x, const Tensor& residual, const Tensor& state
     return y;
 }
 struct Dropout : torch::autograd::Function<Dropout> {
+    // x and residual as the caller has them: a copy made ahead of this node would be a node between it and the leaf (check_backward)
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const OptTensor& state, int64_t dtype,
                           int64_t rows, int64_t cols, int64_t n_z, double p, int64_t seed, int64_t elem_offset, int64_t draw) {
         auto& d = ctx->saved_data;
@@ -92,10 +114,10 @@ struct Dropout : torch::autograd::Function<Dropout> {
         d["p"] = p;
         d["shape"] = x.sizes().vec();
         if (state) ctx->save_for_backward({*state});          // numbers written into it before the backward pass are noticed
-        return drop_forward(x, residual ? *residual : Tensor(), state ? *state : Tensor(), {(int)dtype, rows, cols, (int)n_z, p, (uint64_t)seed, (uint64_t)elem_offset, (int)draw});
+        return drop_forward(x.contiguous(), dense(residual), dense(state), {(int)dtype, rows, cols, (int)n_z, p, (uint64_t)seed, (uint64_t)elem_offset, (int)draw});
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grads) {
-        first_order("dropout");
+        check_backward("dropout");
         const auto c = ctx->saved_data["call"].toIntVector();
         const auto saved = ctx->get_saved_variables();
         torch::autograd::tensor_list out(11);
@@ -110,7 +132,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
         return out;
     }
 };
-Tensor dropout(const Tensor& x, double p, uint64_t seed, const OptTensor& state_, int64_t elem_offset, int64_t draw, int64_t n_z, const OptTensor& residual_) {
+Tensor dropout(const Tensor& x, double p, uint64_t seed, const OptTensor& state_, int64_t elem_offset, int64_t draw, int64_t n_z, const OptTensor& residual) {
     on_gpu(x);
     const int dtype = dtype_of(x, "dropout");
     if (x.dim() < 1) refuse("dropout: x is a scalar; expected (..., cols)");
@@ -122,17 +144,15 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, const OptTensor& state_
             refuse("dropout: a seed tensor holds two int64 numbers on ", x.device().str(), ", got ", state.sizes(), " ", state.scalar_type(), " on ", state.device().str());
     }
     const int64_t cols = x.size(-1);
-    OptTensor residual;
-    if (residual_) {
+    if (residual) {
         auto shape = x.sizes().vec();
         if (n_z > 1) shape.insert(shape.end() - 1, n_z);
-        residual = same(*residual_, x, shape, "dropout: residual");
+        same(*residual, x, shape, "dropout: residual");
     }
-    const Tensor xc = x.contiguous();
-    const int64_t rows = cols ? xc.numel() / cols : 0;
+    const int64_t rows = cols ? x.numel() / cols : 0;
     if (at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad())))
-        return Dropout::apply(xc, residual, state_, (int64_t)dtype, rows, cols, n_z, p, (int64_t)seed, elem_offset, draw);
-    return drop_forward(xc, residual ? *residual : Tensor(), state_ ? *state_ : Tensor(), {dtype, rows, cols, (int)n_z, p, seed, (uint64_t)elem_offset, (int)draw});
+        return Dropout::apply(x, residual, state_, (int64_t)dtype, rows, cols, n_z, p, (int64_t)seed, elem_offset, draw);
+    return drop_forward(x.contiguous(), dense(residual), dense(state_), {dtype, rows, cols, (int)n_z, p, seed, (uint64_t)elem_offset, (int)draw});
 }
 
 // ------------------------------------------------------------------------------------------------ norm
@@ -157,14 +177,15 @@ Normed norm_forward(const Tensor& x, const Tensor& residual, const Tensor& weigh
 }
 struct RmsNorm : torch::autograd::Function<RmsNorm> {
     static torch::autograd::tensor_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const OptTensor& weight, double eps) {
-        const Normed n = norm_forward(x, residual ? *residual : Tensor(), weight ? *weight : Tensor(), eps, false);
-        ctx->save_for_backward({n.h.defined() ? n.h : x, weight ? *weight : Tensor()});
+        const Tensor xc = x.contiguous(), wc = dense(weight);          // the caller's tensors come in, as in Dropout
+        const Normed n = norm_forward(xc, dense(residual), wc, eps, false);
+        ctx->save_for_backward({n.h.defined() ? n.h : xc, wc});
         ctx->saved_data["eps"] = eps;
         ctx->set_materialize_grads(false);
         return n.h.defined() ? torch::autograd::tensor_list{n.y, n.h} : torch::autograd::tensor_list{n.y};
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grads) {
-        first_order("rms_norm");
+        check_backward("rms_norm");
         const auto saved = ctx->get_saved_variables();
         const Tensor h = saved[0], weight = saved[1];
         const Tensor g = grads[0].defined() ? grads[0].contiguous() : Tensor();
@@ -185,35 +206,29 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         return {ctx->needs_input_grad(0) ? dx : Tensor(), residual && ctx->needs_input_grad(1) ? dx : Tensor(), dw, Tensor()};
     }
 };
-struct NormArgs {
-    Tensor x, residual, weight;
-    NormArgs(const char* what, const Tensor& x_, const OptTensor& weight_, const OptTensor& residual_) {
-        on_gpu(x_);
-        dtype_of(x_, what);
-        if (x_.dim() < 1 || x_.size(-1) < 1) refuse(what, ": x has shape ", x_.sizes(), "; expected (..., cols) with cols >= 1");
-        if (weight_) {
-            weight = *weight_;
-            if (weight.dim() != 1 || weight.size(0) != x_.size(-1) || (weight.scalar_type() != at::kFloat && weight.scalar_type() != x_.scalar_type()) ||
-                weight.device() != x_.device())
-                refuse(what, ": weight: expected (", x_.size(-1), ",) ", x_.scalar_type(), " or float32 on ", x_.device().str(), ", got ", weight.sizes(), " ",
-                       weight.scalar_type(), " on ", weight.device().str());
-            weight = weight.contiguous();
-        }
-        if (residual_) residual = same(*residual_, x_, x_.sizes(), c10::str(what, ": residual").c_str());
-        x = x_.contiguous();
+// checks the arguments; whether a gradient is asked for
+bool norm_args(const char* what, const Tensor& x, const OptTensor& weight_, const OptTensor& residual) {
+    on_gpu(x);
+    dtype_of(x, what);
+    if (x.dim() < 1 || x.size(-1) < 1) refuse(what, ": x has shape ", x.sizes(), "; expected (..., cols) with cols >= 1");
+    if (weight_) {
+        const Tensor& weight = *weight_;
+        if (weight.dim() != 1 || weight.size(0) != x.size(-1) || (weight.scalar_type() != at::kFloat && weight.scalar_type() != x.scalar_type()) ||
+            weight.device() != x.device())
+            refuse(what, ": weight: expected (", x.size(-1), ",) ", x.scalar_type(), " or float32 on ", x.device().str(), ", got ", weight.sizes(), " ",
+                   weight.scalar_type(), " on ", weight.device().str());
     }
-    bool wants() const { return at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(residual)); }
-};
+    if (residual) same(*residual, x, x.sizes(), c10::str(what, ": residual").c_str());
+    return at::GradMode::is_enabled() && (x.requires_grad() || (weight_ && weight_->requires_grad()) || (residual && residual->requires_grad()));
+}
 std::vector<Tensor> rms_norm(const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps) {
-    const NormArgs a("rms_norm", x, weight, residual);
-    if (a.wants()) return RmsNorm::apply(a.x, residual ? OptTensor(a.residual) : OptTensor(), weight ? OptTensor(a.weight) : OptTensor(), eps);
-    const Normed n = norm_forward(a.x, a.residual, a.weight, eps, false);
+    if (norm_args("rms_norm", x, weight, residual)) return RmsNorm::apply(x, residual, weight, eps);
+    const Normed n = norm_forward(x.contiguous(), dense(residual), dense(weight), eps, false);
     return n.h.defined() ? std::vector<Tensor>{n.y, n.h} : std::vector<Tensor>{n.y};
 }
 std::vector<Tensor> rms_norm_e4m3(const Tensor& x, const OptTensor& weight, const OptTensor& residual, double eps) {
-    const NormArgs a("rms_norm_e4m3", x, weight, residual);
-    if (a.wants()) refuse("rms_norm_e4m3 has no backward pass; use rms_norm, or torch.no_grad()");
-    const Normed n = norm_forward(a.x, a.residual, a.weight, eps, true);
+    if (norm_args("rms_norm_e4m3", x, weight, residual)) refuse("rms_norm_e4m3 has no backward pass; use rms_norm, or torch.no_grad()");
+    const Normed n = norm_forward(x.contiguous(), dense(residual), dense(weight), eps, true);
     return n.h.defined() ? std::vector<Tensor>{n.y, n.scale, n.h} : std::vector<Tensor>{n.y, n.scale};
 }
 

@@ -2,6 +2,8 @@
 
 Tolerances count roundings: half a step of the output's type on the result (U), and 2^-24 for each 32-bit operation on the
 way, relative to the terms that it adds."""
+import gc
+
 import pytest
 import torch
 
@@ -586,6 +588,57 @@ def test_training_step_in_a_captured_graph():
         graphs[k % 2][0].replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(graphs[k % 2][1], train())), k
+
+
+@pytest.mark.parametrize("name", ["dropout", "norm"])
+@pytest.mark.parametrize("how", ["grad", "backward"])
+def test_captured_backward_beside_an_eager_graph_of_the_same_leaves(name, how):
+    """Refused: the leaves' gradient nodes are on the eager pass's stream.  Without the eager graph, and on two streams of one
+    capture, it runs.  The leaf x does not lie row by row."""
+    x, r, w = rand(64, 40).t().requires_grad_(True), rand(40, 64, seed=1).requires_grad_(True), (1 + 0.1 * rand(64, seed=2)).requires_grad_(True)
+    g = rand(40, 64, seed=3)
+    leaves = (x, r) if name == "dropout" else (x, r, w)
+
+    def forward():
+        return card_amd.dropout(x, 0.3, seed=1, residual=r) if name == "dropout" else card_amd.rms_norm(x, w, residual=r)[0]
+
+    def backward(y):
+        if how == "grad":
+            return torch.autograd.grad(y, leaves, g)
+        y.backward(g)
+        return [t.grad for t in leaves]
+    want = [t.clone() for t in backward(forward())]
+    for t in leaves:
+        t.grad = None
+    eager = forward()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        y = forward()
+        with pytest.raises(RuntimeError, match="before the capture"):
+            backward(y)
+    del eager, y
+    gc.collect()                                         # what the exception's frames held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = backward(forward())
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        forward()
+    for t in leaves:
+        t.grad = None
+    del got
+    graph, two = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        one = forward()                                  # the leaves' gradient nodes are on this stream, the pass on another
+        two.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(two):
+            got = torch.autograd.grad(forward(), leaves, g)
+        torch.cuda.current_stream().wait_stream(two)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
