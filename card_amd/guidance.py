@@ -191,6 +191,8 @@ class QuantGuidanceNet(GuidanceNet):
         most = max(1, _lib.LINEAR4_MAX_ROWS // n_z)
         if n_z > _lib.LINEAR4_MAX_ROWS:
             raise CardError(f"f_phi: n_z={n_z} > {_lib.LINEAR4_MAX_ROWS} with 4-bit weights")
+        if (chain_offset + int(x.shape[0]) * n_z) * max(lin.out_features for _, _, _, lin in self.layers) >= 2 ** 63:
+            raise CardError(f"f_phi: chain_offset={chain_offset} out of range for layers of this width")
         parts = []
         with torch.no_grad():
             for i in range(0, max(1, x.shape[0]), most):

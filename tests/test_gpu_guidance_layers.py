@@ -189,3 +189,5 @@ def test_refusals():
     with pytest.raises(CardError, match="1024"):
         GuidanceNet.from_module(wide)
     assert torch.isfinite(GuidanceNet.from_module(wide, weight_bits=4).forward(x)).all()
+    with pytest.raises(CardError, match="out of range"):          # elements are counted in 63 bits
+        GuidanceNet.from_module(network([13, 3000, 1]).to(DEV), weight_bits=4).mc_dropout(x, 2, seed=1, chain_offset=2 ** 52 - 1)
