@@ -162,7 +162,8 @@ int shape_of(const char* who, int32_t dtype, int64_t rows, int64_t cols, int32_t
     s->small = s->total < (1ll << 31) - 64;
     s->by_cols.set(cols > 0 ? cols : 1);
     s->by_nz.set(n_z);
-    if (all / 16 > (int64_t)kThreads * 0x7ffffff0) return card_fail(CARD_E_UNSUPPORTED, "%s: more than 2^31 workgroups", who);
+    // a launch has fewer than 2^32 threads, and the last workgroup is rounded up
+    if (all / 16 > (1ll << 32) - 4 * kThreads) return card_fail(CARD_E_UNSUPPORTED, "%s: more than 2^24 workgroups (16 bytes a thread)", who);
     return CARD_OK;
 }
 
@@ -189,7 +190,7 @@ template <typename T> int backward(const Shape& s, const DropRule& d, const void
     int lanes = 1;
     while (lanes < 64 && 2 * lanes <= s.n_z && chunks * lanes < 1 << 17) lanes *= 2;
     const long long per_wg = kThreads / lanes, grid = (chunks + per_wg - 1) / per_wg;
-    if (grid > 0x7fffffff) return card_fail(CARD_E_UNSUPPORTED, "card_dropout_backward: more than 2^31 workgroups");
+    if (grid >= 1 << 24) return card_fail(CARD_E_UNSUPPORTED, "card_dropout_backward: more than 2^24 workgroups");
     dropout_backward_kernel<T><<<(unsigned)grid, kThreads, 0, stream>>>(s, by_chunks, d, (const T*)g, (T*)dx, lanes);
     HIP_TRY(hipGetLastError());
     return CARD_OK;

@@ -29,50 +29,53 @@ constexpr int kThreads = 256, kBlock = 128;
 // value of column 2 j + h sits in the word's field j + 4 h; field 0 begins at bit 3 and field 7 wraps around.  A mask then
 // leaves two neighbouring columns as the mantissas of two bf16 numbers 16 + q (bf16_of below) and three shifts give the rest.
 __global__ void pack_kernel(const uint8_t* q, int in, int out_f, int blocks, long long n, uint4* out) {
-    const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
-    if (id >= n) return;
-    const int l = (int)(id & 63), block = (int)((id >> 6) % blocks);
-    const long long o = (id >> 6) / blocks * 16 + (l & 15);
-    uint32_t w[4];
-    for (int s = 0; s < 4; ++s) {
-        uint32_t u = 0;
-        for (int i = 0; i < 8; ++i) {
-            const int k = block * kBlock + 32 * s + 8 * (l >> 4) + i;
-            if (o < out_f && k < in) u |= (uint32_t)(q[o * in + k] & 15u) << (4 * (i / 2 + 4 * (i & 1)));
+    for (long long id = (long long)blockIdx.x * kThreads + threadIdx.x; id < n; id += (long long)gridDim.x * kThreads) {
+        const int l = (int)(id & 63), block = (int)((id >> 6) % blocks);
+        const long long o = (id >> 6) / blocks * 16 + (l & 15);
+        uint32_t w[4];
+        for (int s = 0; s < 4; ++s) {
+            uint32_t u = 0;
+            for (int i = 0; i < 8; ++i) {
+                const int k = block * kBlock + 32 * s + 8 * (l >> 4) + i;
+                if (o < out_f && k < in) u |= (uint32_t)(q[o * in + k] & 15u) << (4 * (i / 2 + 4 * (i & 1)));
+            }
+            w[s] = u << 3 | u >> 29;
         }
-        w[s] = u << 3 | u >> 29;
+        out[id] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    out[id] = make_uint4(w[0], w[1], w[2], w[3]);
 }
 __global__ void side_kernel(const float* scale, const uint8_t* zero, const float* bias, int group, int groups, int blocks, int out_f,
                             long long n, float* s, uint8_t* z, float* b) {
-    const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
-    if (id < out_f) b[id] = bias ? bias[id] : 0.0f;
-    if (id >= n) return;
     const int per = kBlock / group;
-    const long long at = id >> 4, o = at / per / blocks * 16 + (id & 15), g = at % ((long long)per * blocks);
-    const bool real = o < out_f && g < groups;
-    s[id] = real ? scale[o * groups + g] : 0.0f;
-    z[id] = real && zero ? zero[o * groups + g] & 15u : 8u;
+    for (long long id = (long long)blockIdx.x * kThreads + threadIdx.x; id < n; id += (long long)gridDim.x * kThreads) {          // n >= out_f
+        if (id < out_f) b[id] = bias ? bias[id] : 0.0f;
+        const long long at = id >> 4, o = at / per / blocks * 16 + (id & 15), g = at % ((long long)per * blocks);
+        const bool real = o < out_f && g < groups;
+        s[id] = real ? scale[o * groups + g] : 0.0f;
+        z[id] = real && zero ? zero[o * groups + g] & 15u : 8u;
+    }
 }
 
 // one wave per (row o of the weights, group of columns): q = round(w / scale) + zero with scale = (max - min) / 15 over the
 // group's values and zero
 __global__ __launch_bounds__(kThreads) void quantize_kernel(const float* W, int in, int group, int groups, long long n, uint8_t* q,
                                                             float* scale, uint8_t* zero) {
-    const long long id = (long long)blockIdx.x * (kThreads / 64) + threadIdx.x / 64;
-    if (id >= n) return;
     const int lane = threadIdx.x & 63;
-    const long long o = id / groups;
-    const int k0 = (int)(id - o * groups) * group, k1 = k0 + group < in ? k0 + group : in;
-    float lo = 0.0f, hi = 0.0f;
-    for (int k = k0 + lane; k < k1; k += 64) { lo = fminf(lo, W[o * in + k]); hi = fmaxf(hi, W[o * in + k]); }
-    for (int s = 1; s < 64; s <<= 1) { lo = fminf(lo, __shfl_xor(lo, s, 64)); hi = fmaxf(hi, __shfl_xor(hi, s, 64)); }
-    const float sc = (hi - lo) / 15.0f, inv = sc > 0.0f ? 1.0f / sc : 0.0f;
-    const float z = fminf(fmaxf(rintf(-lo * inv), 0.0f), 15.0f);
-    if (lane == 0) { scale[id] = sc; zero[id] = (uint8_t)z; }
-    for (int k = k0 + lane; k < k1; k += 64) q[o * in + k] = (uint8_t)fminf(fmaxf(rintf(W[o * in + k] * inv) + z, 0.0f), 15.0f);
+    for (long long id = (long long)blockIdx.x * (kThreads / 64) + threadIdx.x / 64; id < n; id += (long long)gridDim.x * (kThreads / 64)) {
+        const long long o = id / groups;
+        const int k0 = (int)(id - o * groups) * group, k1 = k0 + group < in ? k0 + group : in;
+        float lo = 0.0f, hi = 0.0f;
+        for (int k = k0 + lane; k < k1; k += 64) { lo = fminf(lo, W[o * in + k]); hi = fmaxf(hi, W[o * in + k]); }
+        for (int s = 1; s < 64; s <<= 1) { lo = fminf(lo, __shfl_xor(lo, s, 64)); hi = fmaxf(hi, __shfl_xor(hi, s, 64)); }
+        const float sc = (hi - lo) / 15.0f, inv = sc > 0.0f ? 1.0f / sc : 0.0f;
+        const float z = fminf(fmaxf(rintf(-lo * inv), 0.0f), 15.0f);
+        if (lane == 0) { scale[id] = sc; zero[id] = (uint8_t)z; }
+        for (int k = k0 + lane; k < k1; k += 64) q[o * in + k] = (uint8_t)fminf(fmaxf(rintf(W[o * in + k] * inv) + z, 0.0f), 15.0f);
+    }
 }
+
+// a launch has fewer than 2^32 threads: what prepares weights walks over them with fewer
+unsigned walkers(long long workgroups) { return (unsigned)(workgroups < 1 << 20 ? workgroups : 1 << 20); }
 
 struct Args {
     const uint4* q;
@@ -471,9 +474,8 @@ extern "C" CARD_API int card_linear4_quantize(const float* W, int32_t out_featur
     if (group != 32 && group != 64 && group != 128) return card_fail(CARD_E_UNSUPPORTED, "%s: group=%d is none of 32, 64, 128", who, group);
     if (!W || !q || !scale || !zero) return card_fail(CARD_E_INVALID, "%s: null argument", who);
     const int groups = (in_features + group - 1) / group;
-    const long long n = (long long)out_features * groups, grid = (n + kThreads / 64 - 1) / (kThreads / 64);
-    if (grid > 0x7fffffff) return card_fail(CARD_E_UNSUPPORTED, "%s: more than 2^31 workgroups", who);
-    quantize_kernel<<<(unsigned)grid, kThreads, 0, (hipStream_t)stream>>>(W, in_features, group, groups, n, q, scale, zero);
+    const long long n = (long long)out_features * groups;
+    quantize_kernel<<<walkers((n + kThreads / 64 - 1) / (kThreads / 64)), kThreads, 0, (hipStream_t)stream>>>(W, in_features, group, groups, n, q, scale, zero);
     HIP_TRY(hipGetLastError());
     return CARD_OK;
 }
@@ -502,13 +504,13 @@ extern "C" CARD_API int card_linear4_create(const card_linear4_desc* d, void* st
     if (e == hipSuccess) e = hipMalloc(&s->zero, ng);
     if (e == hipSuccess) e = hipMalloc(&s->bias, s->out * sizeof(float));
     if (e == hipSuccess) {
-        const long long ns = ng > s->out ? ng : s->out;
-        pack_kernel<<<(unsigned)((nw + kThreads - 1) / kThreads), kThreads, 0, st>>>(d->q, s->in, s->out, s->blocks, nw, s->q);
-        side_kernel<<<(unsigned)((ns + kThreads - 1) / kThreads), kThreads, 0, st>>>(d->scale, d->zero, d->bias, s->group, (s->in + s->group - 1) / s->group,
+        pack_kernel<<<walkers((nw + kThreads - 1) / kThreads), kThreads, 0, st>>>(d->q, s->in, s->out, s->blocks, nw, s->q);
+        side_kernel<<<walkers((ng + kThreads - 1) / kThreads), kThreads, 0, st>>>(d->scale, d->zero, d->bias, s->group, (s->in + s->group - 1) / s->group,
                                                                                   s->blocks, s->out, ng, s->scale, s->zero, s->bias);
         e = hipGetLastError();
     }
     if (e != hipSuccess) {
+        (void)hipGetLastError();                         // or the next launch's check would find it
         card_linear4_destroy(s);
         return card_fail(e == hipErrorOutOfMemory ? CARD_E_NOMEM : CARD_E_HIP, "%s: %s", who, hipGetErrorString(e));
     }

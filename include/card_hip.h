@@ -342,7 +342,7 @@ typedef enum card_dtype {
  * x (rows, cols); residual (rows, n_z, cols) or NULL; out (rows, n_z, cols): n_z masks of every row, as the sampler's n_z.
  * keep(e): word e & 3 of Philox4x32-10 at counter (low and high word of e >> 2, draw, 1) under the key `seed` is at least
  * round(p * 2^32).  (The sampler's normals use 0 as the last counter word: one seed serves both.)  A dropped element is 0
- * whatever x holds there; p = 1 drops everything.  state: NULL, or two device words {seed, element offset} that are read
+ * whatever x holds there; p = 1 drops everything.  One call's output has less than 64 GiB.  state: NULL, or two device words {seed, element offset} that are read
  * when the kernel runs: the seed replaces `seed`, the offset is added to elem_offset (a captured graph then draws a new mask
  * whenever the words change).  dtype: CARD_DTYPE_F32, _BF16, _F16; sums are fp32, rounded once.  0 <= p <= 1, draw >= 0,
  * elem_offset < 2^63. */
@@ -357,7 +357,8 @@ CARD_API int card_dropout_backward(const void* g, void* dx, int32_t dtype, int64
  * F16); residual and h are both given or both NULL (then h is x).  weight: (cols) floats or of `dtype`, NULL = ones.
  * y_dtype = dtype: y is (rows, cols) of that type and scale is NULL.  y_dtype = CARD_DTYPE_E4M3: scale[row] = max |y| / 448
  * (floats, (rows)) and y holds y / scale[row] in 8 bits; a row of zeros has scale 0, a row with a NaN is NaN throughout.
- * y and scale come from h before h is rounded to its type.  cols <= CARD_NORM_MAX_COLS. */
+ * y and scale come from h before h is rounded to its type; squares are summed in floats, so rows with |h| of 2^60 and more
+ * overflow there.  cols <= CARD_NORM_MAX_COLS. */
 #define CARD_NORM_MAX_COLS 65536
 CARD_API int card_rms_norm(const void* x, const void* residual, const void* weight, int32_t dtype, int32_t weight_dtype, int64_t rows,
                            int64_t cols, double eps, void* h, void* y, int32_t y_dtype, float* scale, void* stream);

@@ -453,6 +453,30 @@ def test_quantize_weight(group):
     assert torch.equal(lin(x), card_amd.QuantLinear(q, s, z, group=group)(x))
 
 
+def test_quantize_weight_of_more_groups_than_a_launch_has_waves():
+    rows, cols = 1 << 21, 1024                   # 2^26 groups, a wave each
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    w = torch.randn(rows, cols, device=DEV, generator=gen)
+    whole = card_amd.quantize_weight(w, group=32)
+    for part in (slice(0, 64), slice(rows // 2 - 32, rows // 2 + 32), slice(rows - 64, rows)):
+        for a, b in zip(whole, card_amd.quantize_weight(w[part].contiguous(), group=32)):
+            assert torch.equal(a[part], b)
+    assert bool((whole[1] > 0).all())
+
+
+def test_weights_that_do_not_fit_leave_no_error_behind():
+    """549 GB of weights are refused by the allocator, before anything is launched; the next call is none the worse."""
+    import ctypes as C
+    from card_amd import _lib
+    d, h, t = _lib.Linear4Desc(), C.c_void_p(), torch.zeros(16, device=DEV)
+    d.struct_bytes, d.in_features, d.out_features, d.group = C.sizeof(_lib.Linear4Desc), _lib.LINEAR4_MAX_FEATURES, _lib.LINEAR4_MAX_FEATURES, 128
+    d.q = d.scale = t.data_ptr()
+    assert _lib.lib().card_linear4_create(C.byref(d), None, C.byref(h)) != 0 and not h.value
+    x = rand(4, 64)
+    assert torch.equal(card_amd.dropout(x, 0.0, seed=1), x)
+    torch.cuda.synchronize()
+
+
 # ------------------------------------------------------------------------------------------------ together
 def test_a_layer_as_it_is_served_and_trained():
     """residual -> norm -> 8 bits -> 4-bit product -> LeakyReLU, and the training form of its ends: norm, dropout."""

@@ -23,6 +23,7 @@ def msg():
     (dict(n_z=0), E_INVALID, "n_z"), (dict(p=-0.1), E_INVALID, "p="), (dict(p=1.1), E_INVALID, "p="), (dict(p=float("nan")), E_INVALID, "p="),
     (dict(draw=-1), E_INVALID, "draw"), (dict(elem_offset=1 << 63), E_INVALID, "elem_offset"), (dict(x=None), E_INVALID, "null"), (dict(out=None), E_INVALID, "null"),
     (dict(rows=1 << 40, cols=1 << 30), E_INVALID, "63 bits"), (dict(rows=1 << 30, cols=1 << 20, n_z=1 << 5), E_UNSUPPORTED, "workgroups"),
+    (dict(rows=1 << 24, cols=1 << 10), E_UNSUPPORTED, "workgroups"), (dict(dtype=2, rows=1 << 25, cols=1 << 10), E_UNSUPPORTED, "workgroups"),
 ])
 def test_dropout_refusals(change, code, needle):
     L = _lib.lib()
@@ -32,6 +33,12 @@ def test_dropout_refusals(change, code, needle):
     assert L.card_dropout(a["x"], None, a["out"], *tail) == code and needle in msg(), msg()
     if "workgroups" not in needle:          # backward takes a workgroup per chunk of x, not of the masks
         assert L.card_dropout_backward(a["x"], a["out"], *tail) == code and needle in msg(), msg()
+
+
+def test_dropout_backward_of_many_short_rows_is_refused():
+    """A thread for each 16 bytes of dx and no fewer than one to a row: 2^32 of them are no launch."""
+    L = _lib.lib()
+    assert L.card_dropout_backward(P, P, _lib.DTYPE_BF16, 1 << 32, 1, 2, 0.5, 1, 0, None, 0, None) == E_UNSUPPORTED and "workgroups" in msg(), msg()
 
 
 def test_nothing_to_do_is_no_error():
