@@ -226,7 +226,11 @@ template <int G, int NT, bool STREAM> struct Weights {
 };
 
 // acc += one block: per group of columns the matrix pipe forms P = sum (16 + q) x and, against ones, S = sum x (for all NT
-// tiles), the vector pipe adds scale * (P - (16 + zero) S).  part(m, s, k): the k-th part of step s of rows 16 m ...
+// tiles), the vector pipe adds scale * (P - (16 + zero) S).  part(m, s, p): the parts of step s of rows 16 m ...
+// fp32 rows: P and S are some five times their difference, and sums over a group lose that much at their last bit.  So the
+// first part's P and S, products of 13 bits, are taken for 32 columns each, where next to nothing is rounded; only the smaller
+// parts' run over the group.  Off by (root mean square) 6.7e-8 instead of 5.6e-7 at 465 columns, 1.1e-7 and 9.1e-7 at 4096, a
+// plain fp32 product 1.9e-7 and 5.8e-7; it costs 16 rows of 8192 x 28672 52.6 us for 44.5, of 4096 x 4096 8.9 for 8.3.
 template <int X, int G, int MT, int NT, bool STREAM, typename F>
 __device__ __forceinline__ void add_block(const Weights<G, NT, STREAM>& w, uint32_t sixteen, f32x4 (&acc)[MT][NT], F part) {
     constexpr int P = Row8<X>::kParts, S = 4 / G;          // S steps of 32 columns in a group
@@ -235,6 +239,9 @@ __device__ __forceinline__ void add_block(const Weights<G, NT, STREAM>& w, uint3
 #pragma unroll
     for (int g = 0; g < G; ++g) {
         f32x4 sum[MT], prod[MT][NT];
+        float off[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) off[t] = -16.0f - (float)w.z[t][g];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             sum[m] = f32x4{0, 0, 0, 0};
@@ -251,20 +258,28 @@ __device__ __forceinline__ void add_block(const Weights<G, NT, STREAM>& w, uint3
                 u32x4 p[P];
                 part(m, s, p);
 #pragma unroll
-                for (int k = P - 1; k >= 0; --k) {          // the small parts first
+                for (int k = P - 1; k >= (P > 1); --k) {
 #pragma unroll
                     for (int t = 0; t < NT; ++t) prod[m][t] = mfma<X>(p[k], v[t], prod[m][t]);
                     sum[m] = mfma<X>(p[k], ones, sum[m]);
+                }
+                if constexpr (P > 1) {
+                    const f32x4 none = {0, 0, 0, 0}, s0 = mfma<X>(p[0], ones, none);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const f32x4 p0 = mfma<X>(p[0], v[t], none);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(w.s[t][g], fmaf(off[t], s0[r], p0[r]), acc[m][t][r]);
+                    }
                 }
             }
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const float off = -16.0f - (float)w.z[t][g], sc = w.s[t][g];
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(sc, fmaf(off, sum[m][r], prod[m][t][r]), acc[m][t][r]);
+                for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(w.s[t][g], fmaf(off[t], sum[m][r], prod[m][t][r]), acc[m][t][r]);
         }
     }
 }
@@ -446,8 +461,7 @@ int splits_of(int tiles, int blocks, int64_t rows, int x_dtype) {
 // 10.3).  From 1024 tiles on the weights pass by the caches, which cannot hold them (16 rows of 8192 columns, 28672 outputs:
 // 29.7 us against 31.5; but 5.8 against 5.1 for 4096 x 4096, whose weights stay in L2 from call to call), and workgroups are
 // plenty: four tiles and four waves with one block on its way, so that a CU holds four workgroups (8192 columns, 28672
-// outputs: 16 rows bf16 30.2 us against 34.8 with two tiles, eight waves and two blocks, fp32 45.3 and 68.0, 32 rows e4m3
-// 40.0 and 51.1).  Up to 16 rows of e4m3, half of bf16's x to read, need only three tiles to share them, and smaller workgroups
+// outputs: 16 rows bf16 30.2 us against 34.8 with two tiles, eight waves and two blocks, 32 rows e4m3 40.0 and 51.1).  Up to 16 rows of e4m3, half of bf16's x to read, need only three tiles to share them, and smaller workgroups
 // even out the last ones (28672 outputs 29.4 us against 29.9 with four, 17000 outputs of 4096 columns 12.2 and 14.5; but bf16
 // 33.0 against 30.2).
 constexpr int kCus = 256, kStreamTiles = 1024;

@@ -376,6 +376,18 @@ def test_linear4(dtype, group, rows, in_f, out_f):
     assert torch.equal(nob.forward(moved, xs), nob.forward(x, xs))
 
 
+@pytest.mark.parametrize("rows,in_f,out_f,group", [(13, 465, 13, 128), (1, 4096, 512, 128), (60, 70, 9, 64), (24, 4096, 5000, 32), (20, 2048, 16400, 64)])
+def test_linear4_fp32_is_as_exact_as_an_fp32_product(rows, in_f, out_f, group):
+    """The sums of 16 + q on the way cost nothing: a result is off like one that is rounded once for 32 columns and once for a
+    group (half a step each, at random), root mean square."""
+    q, s, z, b = weights(out_f, in_f, group, True)
+    x = rand(rows, in_f, seed=5)
+    want, _ = ref.linear4(q, s, z, None, group, x)
+    y = card_amd.QuantLinear(q, s, z, group=group)(x).cpu().double()
+    n = -(-in_f // 32) + -(-in_f // group)
+    assert float((y - want).norm() / want.norm()) <= n ** 0.5 * U32
+
+
 def test_linear4_row_results_do_not_depend_on_their_neighbours():
     q, s, z, b = weights(200, 640, 64, True)
     lin = card_amd.QuantLinear(q, s, z, b, group=64)
