@@ -239,9 +239,6 @@ __device__ __forceinline__ void add_block(const Weights<G, NT, STREAM>& w, uint3
 #pragma unroll
     for (int g = 0; g < G; ++g) {
         f32x4 sum[MT], prod[MT][NT];
-        float off[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) off[t] = -16.0f - (float)w.z[t][g];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             sum[m] = f32x4{0, 0, 0, 0};
@@ -267,19 +264,21 @@ __device__ __forceinline__ void add_block(const Weights<G, NT, STREAM>& w, uint3
                     const f32x4 none = {0, 0, 0, 0}, s0 = mfma<X>(p[0], ones, none);
 #pragma unroll
                     for (int t = 0; t < NT; ++t) {
+                        const float off = -16.0f - (float)w.z[t][g];
                         const f32x4 p0 = mfma<X>(p[0], v[t], none);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(w.s[t][g], fmaf(off[t], s0[r], p0[r]), acc[m][t][r]);
+                        for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(w.s[t][g], fmaf(off, s0[r], p0[r]), acc[m][t][r]);
                     }
                 }
             }
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+            const float off = -16.0f - (float)w.z[t][g], sc = w.s[t][g];
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(w.s[t][g], fmaf(off[t], sum[m][r], prod[m][t][r]), acc[m][t][r]);
+                for (int r = 0; r < 4; ++r) acc[m][t][r] = fmaf(sc, fmaf(off, sum[m][r], prod[m][t][r]), acc[m][t][r]);
         }
     }
 }
@@ -461,9 +460,9 @@ int splits_of(int tiles, int blocks, int64_t rows, int x_dtype) {
 // 10.3).  From 1024 tiles on the weights pass by the caches, which cannot hold them (16 rows of 8192 columns, 28672 outputs:
 // 29.7 us against 31.5; but 5.8 against 5.1 for 4096 x 4096, whose weights stay in L2 from call to call), and workgroups are
 // plenty: four tiles and four waves with one block on its way, so that a CU holds four workgroups (8192 columns, 28672
-// outputs: 16 rows bf16 30.2 us against 34.8 with two tiles, eight waves and two blocks, 32 rows e4m3 40.0 and 51.1).  Up to 16 rows of e4m3, half of bf16's x to read, need only three tiles to share them, and smaller workgroups
-// even out the last ones (28672 outputs 29.4 us against 29.9 with four, 17000 outputs of 4096 columns 12.2 and 14.5; but bf16
-// 33.0 against 30.2).
+// outputs: 16 rows bf16 30.2 us against 34.8 with two tiles, eight waves and two blocks, 32 rows e4m3 40.0 and 51.1).  Up to
+// 16 rows of e4m3, half of bf16's x to read, need only three tiles to share them, and smaller workgroups even out the last ones
+// (28672 outputs 29.4 us against 29.9 with four, 17000 outputs of 4096 columns 12.2 and 14.5; but bf16 33.0 against 30.2).
 constexpr int kCus = 256, kStreamTiles = 1024;
 template <int X, int G, int MT> int by_tiles(const Args& a, const void* x, void* y, hipStream_t st) {
     // blocks on their way: one where rows are wide -- more than 16, or fp32 with its three operands -- for the registers' sake
