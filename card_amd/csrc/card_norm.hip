@@ -276,7 +276,8 @@ __global__ __launch_bounds__(L ? kThreads : 1024, V == 1 && sizeof(F) == 4 ? 6 :
             ss = waves_reduce(buf[turn][0], add);
             sg = waves_reduce(buf[turn][1], add);
         }
-        const F rstd2 = (F)1 / (ss / (F)a.cols + (F)a.eps), rstd = sqrt(rstd2), k = rstd2 * sg / (F)a.cols;
+        // a place behind the last row holds zeros, whose root is infinite where eps is 0: it adds nothing to dw
+        const F rstd2 = live ? (F)1 / (ss / (F)a.cols + (F)a.eps) : (F)0, rstd = sqrt(rstd2), k = rstd2 * sg / (F)a.cols;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const int c = (v * threads + t) * N, n = live ? a.cols - c : 0;
