@@ -1,7 +1,7 @@
 // card_norm.hip - root-mean-square norm of rows, with the residual's addition before it and 8 bits after it.
 //
 //   h = x + residual,  y = h * rstd * w,  rstd = 1 / sqrt(mean(h^2) + eps)
-//   8 bits: amax = max |y| of the row, scale = amax / 448, q = e4m3(y * 448 / amax)     (y itself is never stored)
+//   8 bits: amax = max |y| of the row, scale = max(amax / 448, 2^-140), q = e4m3(y / scale)     (y itself is never stored)
 //   backward, from the h that forward stored:  gw = g * w,  dx = rstd * (gw - h * rstd^2 * mean(gw * h)) + gh,
 //   dw = sum over rows of g * h * rstd;  the residual's gradient is dx.
 //
@@ -202,9 +202,19 @@ __global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_kernel(const Nor
         }
         if constexpr (Q) {
             amax = row_reduce<L>(amax, buf[turn][1], max_nan);
-            // a row of zeros (or of values below 448 / FLT_MAX) must not divide by zero; NaN stays NaN
-            const float inv = amax < 1.4e-36f ? 3.0e38f : kE4m3Max / amax;
-            if (live && t == 0) a.scale[row] = amax / kE4m3Max;
+            // scale is 2^-140 at least, which a float holds to 2^-10 and where the smallest of them, 2^-149, is still a number of 8
+            // bits.  448 / amax passes the largest float in rows below 1.4e-36: those are lifted by 2^100 first, which is exact, and
+            // divided by the scale as it was rounded.  (A row of zeros has scale 0; NaN stays NaN.)
+            const float scale = amax > 0.0f ? fmaxf(amax / kE4m3Max, 0x1p-140f) : amax;
+            float inv = kE4m3Max / amax;
+            if (amax < 1.4e-36f) {
+                inv = amax > 0.0f ? 1.0f / (scale * 0x1p100f) : 0.0f;
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) h[v][i] *= 0x1p100f;
+            }
+            if (live && t == 0) a.scale[row] = scale;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const int c = (v * threads + t) * N, n = live ? a.cols - c : 0;

@@ -63,7 +63,7 @@ def rms_norm(x, weight=None, *, residual=None, eps=1e-6):
 
 def rms_norm_e4m3(x, weight=None, *, residual=None, eps=1e-6):
     """rms_norm with its result in 8 bits: (q, scale) or (q, scale, h), with q float8_e4m3fn and scale (...,) float32, so that
-    q * scale[..., None] stands for y; scale = max |y| / 448 of each row.  What QuantLinear takes as (x, x_scale)."""
+    q * scale[..., None] stands for y; scale = max |y| / 448 of each row (2^-140 at least; 0 for a row of zeros).  What QuantLinear takes as (x, x_scale)."""
     return tuple((_ext or _load()).rms_norm_e4m3(x, weight, residual, eps))
 
 

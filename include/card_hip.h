@@ -355,10 +355,11 @@ CARD_API int card_dropout_backward(const void* g, void* dx, int32_t dtype, int64
 
 /* h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight, row by row.  x, residual, h: (rows, cols) of `dtype` (F32, BF16,
  * F16); residual and h are both given or both NULL (then h is x).  weight: (cols) floats or of `dtype`, NULL = ones.
- * y_dtype = dtype: y is (rows, cols) of that type and scale is NULL.  y_dtype = CARD_DTYPE_E4M3: scale[row] = max |y| / 448
- * (floats, (rows)) and y holds y / scale[row] in 8 bits; a row of zeros has scale 0, a row with a NaN is NaN throughout.
- * y and scale come from h before h is rounded to its type; squares are summed in floats, so rows with |h| of 2^60 and more
- * overflow there.  cols <= CARD_NORM_MAX_COLS. */
+ * y_dtype = dtype: y is (rows, cols) of that type and scale is NULL.  y_dtype = CARD_DTYPE_E4M3: scale[row] = max |y| / 448,
+ * but 2^-140 at least (floats, (rows)), and y holds y / scale[row] in 8 bits; a row of zeros has scale 0, a row with a NaN is NaN
+ * throughout.
+ * y and scale come from h before h is rounded to its type; squares are summed in floats: rows are right for |h| below 2^60 and,
+ * where eps does not outweigh it, above 2^-60.  cols <= CARD_NORM_MAX_COLS. */
 #define CARD_NORM_MAX_COLS 65536
 CARD_API int card_rms_norm(const void* x, const void* residual, const void* weight, int32_t dtype, int32_t weight_dtype, int64_t rows,
                            int64_t cols, double eps, void* h, void* y, int32_t y_dtype, float* scale, void* stream);
