@@ -293,6 +293,38 @@ __device__ __forceinline__ void store_y(const Args& a, void* y, long long at, fl
     else ((f16_t*)y)[at] = (f16_t)v;
 }
 
+template <int X> __device__ __forceinline__ float value_of(typename Row8<X>::elem v) {
+    if constexpr (X == CARD_DTYPE_F32) return __uint_as_float(v);
+    else if constexpr (X == CARD_DTYPE_BF16) return __uint_as_float((uint32_t)v << 16);
+    else if constexpr (X == CARD_DTYPE_F16) return (float)__builtin_bit_cast(_Float16, v);
+    else return __builtin_amdgcn_cvt_f32_fp8((int)v, 0);
+}
+// One sum as it is defined, weight by weight, where the sum by P and S is not finite: an infinite x makes both infinite and
+// their difference NaN, and x of 2^115 and more passes the largest float there.  A thread to an output, 128 columns at a time;
+// a NaN ends it.
+template <int X, int G> __device__ float plain_sum(const Args& a, const typename Row8<X>::elem* x, int row, long long o) {
+    const typename Row8<X>::elem* xr = x + (long long)row * a.in;
+    float sum = 0.0f;
+    for (int b = 0; b < a.blocks && sum == sum; ++b) {
+        const long long i = (o >> 4) * a.blocks + b;
+        float part = 0.0f;
+#pragma unroll 4
+        for (int c = 0; c < 16; ++c) {                   // columns 8 c ... of the block: lanes 16 (c % 4) ..., word c / 4
+            const long long at = (i * G + c * G / 16) * 16 + (o & 15);
+            const uint32_t w = ((const uint32_t*)a.q)[(i * 64 + 16 * (c & 3) + (o & 15)) * 4 + (c >> 2)], u = w >> 3 | w << 29;
+            const float s = a.scale[at], z = (float)a.zero[at];
+            const int k = b * kBlock + 8 * c;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = value_of<X>(xr[k + j < a.in ? k + j : a.in - 1]), n = (float)(u >> (4 * (j / 2 + 4 * (j & 1))) & 15u);
+                part += k + j < a.in ? (n - z) * s * v : 0.0f;
+            }
+        }
+        sum += part;
+    }
+    return sum;
+}
+
 // What the epilogue multiplies and adds for one output: asked for at the start, so that it has come by the end.
 struct Out {
     int row;
@@ -311,8 +343,8 @@ struct Out {
 };
 
 // The waves join through LDS in a fixed order, and the epilogue.
-template <int MT, int NT>
-__device__ __forceinline__ void finish(const Args& a, const f32x4 (&acc)[MT][NT], float* join, int tile0, int m0, Out out, void* y) {
+template <int X, int G, int MT, int NT>
+__device__ __forceinline__ void finish(const Args& a, const typename Row8<X>::elem* x, const f32x4 (&acc)[MT][NT], float* join, int tile0, int m0, Out out, void* y) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -328,19 +360,25 @@ __device__ __forceinline__ void finish(const Args& a, const f32x4 (&acc)[MT][NT]
         float v = join[id];
         for (int w = 1; w < waves; ++w) v += join[w * n + id];
         const long long at = (long long)out.row * a.out + out.o;
-        if (a.partial) a.partial[(long long)blockIdx.z * a.rows * a.out + at] = v;
-        else store_y(a, y, at, epilogue(a, v, out.x_scale, out.bias, out.gamma));
+        if (a.partial) {
+            a.partial[(long long)blockIdx.z * a.rows * a.out + at] = v;
+        } else {
+            if (!__builtin_isfinite(v)) v = plain_sum<X, G>(a, x, out.row, out.o);
+            store_y(a, y, at, epilogue(a, v, out.x_scale, out.bias, out.gamma));
+        }
     }
 }
 
 // the shares of the columns join in a fixed order
-__global__ __launch_bounds__(kThreads) void linear4_join_kernel(const Args a, void* y) {
+template <int X, int G>
+__global__ __launch_bounds__(kThreads) void linear4_join_kernel(const Args a, const typename Row8<X>::elem* x, void* y) {
     const long long id = (long long)blockIdx.x * kThreads + threadIdx.x, n = (long long)a.rows * a.out;
     if (id >= n) return;
     const int row = (int)(id / a.out), o = (int)(id - (long long)row * a.out);
     float v = a.partial[id];
 #pragma unroll 4
     for (int k = 1; k < a.splits; ++k) v += a.partial[k * n + id];
+    if (!__builtin_isfinite(v)) v = plain_sum<X, G>(a, x, row, o);
     store_y(a, y, id, epilogue(a, v, a.x_scale ? a.x_scale[row] : 1.0f, a.bias[o], a.gamma ? a.gamma[o] : 1.0f));
 }
 
@@ -429,17 +467,18 @@ __global__ __launch_bounds__(64 * WAVES) void linear4_kernel(const Args a, const
             for (int s = 0; s < 4; ++s) st[0].x[m][s] = load_tail<X>(xr[m] - lcol, b1 * kBlock + 32 * s + lcol, a.in);
         use(st[0]);
     }
-    finish<MT, NT>(a, acc, join, tile0, m0, out, y);
+    finish<X, G, MT, NT>(a, x, acc, join, tile0, m0, out, y);
 }
 
 template <int X, int G, int MT, int NT, int U, bool STREAM, int WAVES> int launch(const Args& a, const void* x, void* y, hipStream_t st) {
     int waves = 1;                                   // a block of columns for each at least
     while (waves < WAVES && a.blocks / a.splits >= 2 * waves) waves *= 2;
     const dim3 grid((a.tiles + NT - 1) / NT, (a.rows + 16 * MT - 1) / (16 * MT), a.splits);
-    linear4_kernel<X, G, MT, NT, U, STREAM, WAVES><<<grid, 64 * waves, waves * NT * MT * 256 * sizeof(float), st>>>(a, (const typename Row8<X>::elem*)x, y);
+    const typename Row8<X>::elem* xe = (const typename Row8<X>::elem*)x;
+    linear4_kernel<X, G, MT, NT, U, STREAM, WAVES><<<grid, 64 * waves, waves * NT * MT * 256 * sizeof(float), st>>>(a, xe, y);
     HIP_TRY(hipGetLastError());
     if (a.partial) {
-        linear4_join_kernel<<<(unsigned)(((long long)a.rows * a.out + kThreads - 1) / kThreads), kThreads, 0, st>>>(a, y);
+        linear4_join_kernel<X, G><<<(unsigned)(((long long)a.rows * a.out + kThreads - 1) / kThreads), kThreads, 0, st>>>(a, xe, y);
         HIP_TRY(hipGetLastError());
     }
     return CARD_OK;

@@ -392,8 +392,8 @@ CARD_API void card_linear4_destroy(card_linear4* s);
 /* y[m, o] = act(gamma[o] * (x_scale[m] * sum_k w[o, k] x[m, k] + bias[o])), act(v) = v > 0 ? v : slope * v.
  * x (rows, in) of any card_dtype; x_scale (rows) goes with CARD_DTYPE_E4M3 and is NULL otherwise; gamma (out) or NULL = ones
  * (a ConditionalLinear's embed.weight[t], regression/model.py:16-17); slope 1 = no activation; y (rows, out) F32, BF16 or F16.
- * Made for one to some tens of rows; at most CARD_LINEAR4_MAX_ROWS.  The weights' device must be current.  On the way sums hold
- * up to 31 times the magnitudes of x over a group: x of 2^115 and more may overflow there.
+ * Made for one to some tens of rows; at most CARD_LINEAR4_MAX_ROWS.  The weights' device must be current.  Sums that are not finite
+ * on the way (an infinite x, or x of 2^115 and more) are formed again weight by weight, which is slower.
  * workspace: card_linear4_workspace_bytes of scratch (0 for most shapes; then NULL is fine), 16-byte aligned; calls that share
  * one must not overlap in time. */
 CARD_API int card_linear4_workspace_bytes(const card_linear4* s, int32_t x_dtype, int64_t rows, uint64_t* bytes);

@@ -5,7 +5,7 @@ import torch
 import card_amd
 from tests import layer_reference as ref
 from tests.layer_reference import TINY, U, U32, assert_within
-from tests.test_gpu_layers import DEV, TYPES, chain, ids, rand
+from tests.test_gpu_layers import DEV, TYPES, chain, ids, lin_bound, rand, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,42 @@ def test_rms_norm_e4m3_of_tiny_rows(dtype, cols):
     assert bool((q.float().abs().amax(-1).cpu()[amax > 2.0 ** -131] == 448).all())          # 448 * 2^-140 < 2^-131
     zero = card_amd.rms_norm_e4m3(torch.zeros(2, cols, device=DEV, dtype=dtype), eps=1.0)
     assert bool((zero[1] == 0).all()) and bool((zero[0].float() == 0).all())
+
+
+# ------------------------------------------------------------------------------------------------ 4-bit weights
+# (20, 12300, 24): the columns in shares; (4, 129, 16400): weights past the caches
+INF_SHAPES = [(4, 31, 33), (5, 200, 40), (20, 136, 5000), (4, 129, 16400), (20, 12300, 24)]
+
+
+@pytest.mark.parametrize("rows,in_f,out_f", INF_SHAPES)
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_linear4_infinite_rows(dtype, group, rows, in_f, out_f):
+    """An infinite x is an infinity of the weight's sign in every output, NaN where the weight is 0 or infinities meet."""
+    q, s, z, b = weights(out_f, in_f, group, True)
+    lin = card_amd.QuantLinear(q, s, z, b, group=group)
+    x = rand(rows, in_f, seed=5, dtype=dtype)
+    clean = lin.forward(x, out_dtype=torch.float32)
+    bad = x.clone()
+    bad[0, 5], bad[1, in_f - 1] = float("inf"), -float("inf")
+    bad[2, 3], bad[2, 30] = float("inf"), float("inf")
+    for gamma, slope in ((None, None), (rand(out_f, seed=6), 0.01)):
+        want, size = ref.linear4(q, s, z, b, group, bad, None, gamma, slope)
+        y = lin.forward(bad, gamma=gamma, slope=slope, out_dtype=torch.float32)
+        assert_within(y, want, lin_bound(want, size, group, in_f, torch.float32))
+        assert bool(torch.isinf(y[0]).any())
+    assert torch.equal(lin.forward(bad, out_dtype=torch.float32)[3:], clean[3:])
+
+
+@pytest.mark.parametrize("rows,in_f,out_f", INF_SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids)
+def test_linear4_rows_near_the_end_of_the_range(dtype, rows, in_f, out_f):
+    """Finite rows whose sums with 16 + q pass the largest float, results that do not."""
+    q, s, z, b = weights(out_f, in_f, 64, True)
+    s = s * 2.0 ** -10
+    lin = card_amd.QuantLinear(q, s, z, b, group=64)
+    x = (rand(rows, in_f, seed=5).clamp(-3.9, 3.9) * 2.0 ** 126).to(dtype)
+    x[-1] = 1.0
+    want, size = ref.linear4(q, s, z, b, 64, x)
+    assert bool((want.abs() < 2.0 ** 127).all())
+    assert_within(lin.forward(x, out_dtype=torch.float32), want, lin_bound(want, size, 64, in_f, torch.float32))
