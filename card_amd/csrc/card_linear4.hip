@@ -57,7 +57,7 @@ __global__ void side_kernel(const float* scale, const uint8_t* zero, const float
 }
 
 // one wave per (row o of the weights, group of columns): q = round(w / scale) + zero with scale = (max - min) / 15 over the
-// group's values and zero
+// group's values and zero.  A NaN or an infinity makes the scale NaN or infinite, and so the group: q - zero is 0 then.
 __global__ __launch_bounds__(kThreads) void quantize_kernel(const float* W, int in, int group, int groups, long long n, uint8_t* q,
                                                             float* scale, uint8_t* zero) {
     const int lane = threadIdx.x & 63;
@@ -65,12 +65,25 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const float* W, int 
         const long long o = id / groups;
         const int k0 = (int)(id - o * groups) * group, k1 = k0 + group < in ? k0 + group : in;
         float lo = 0.0f, hi = 0.0f;
-        for (int k = k0 + lane; k < k1; k += 64) { lo = fminf(lo, W[o * in + k]); hi = fmaxf(hi, W[o * in + k]); }
+        bool nan = false;
+        for (int k = k0 + lane; k < k1; k += 64) {
+            const float w = W[o * in + k];
+            nan |= w != w;
+            lo = fminf(lo, w);
+            hi = fmaxf(hi, w);
+        }
         for (int s = 1; s < 64; s <<= 1) { lo = fminf(lo, __shfl_xor(lo, s, 64)); hi = fmaxf(hi, __shfl_xor(hi, s, 64)); }
-        const float sc = (hi - lo) / 15.0f, inv = sc > 0.0f ? 1.0f / sc : 0.0f;
-        const float z = fminf(fmaxf(rintf(-lo * inv), 0.0f), 15.0f);
+        float sc = (hi - lo) / 15.0f;
+        if (isinf(sc)) sc = hi / 15.0f - lo / 15.0f;                      // the span alone may pass the largest float
+        if (__any(nan)) sc = __builtin_nanf("");
+        const float inv = sc > 0.0f ? 1.0f / sc : 0.0f;
+        const bool tiny = isinf(inv);                                     // a scale whose reciprocal is no float: divide
+        const float z = fminf(fmaxf(rintf(tiny ? -lo / sc : -lo * inv), 0.0f), 15.0f);
         if (lane == 0) { scale[id] = sc; zero[id] = (uint8_t)z; }
-        for (int k = k0 + lane; k < k1; k += 64) q[o * in + k] = (uint8_t)fminf(fmaxf(rintf(W[o * in + k] * inv) + z, 0.0f), 15.0f);
+        for (int k = k0 + lane; k < k1; k += 64) {
+            const float w = W[o * in + k];
+            q[o * in + k] = (uint8_t)(isfinite(sc) ? fminf(fmaxf(rintf(tiny ? w / sc : w * inv) + z, 0.0f), 15.0f) : z);
+        }
     }
 }
 

@@ -401,7 +401,8 @@ CARD_API int card_linear4_forward(const card_linear4* s, const void* x, int32_t 
                                   const float* gamma, float slope, void* y, int32_t y_dtype, void* workspace, uint64_t workspace_bytes,
                                   void* stream);
 /* The nearest such weights of W (out, in) floats: per group scale = (max - min) / 15 over its values and 0, zero = round(-min /
- * scale), q = round(w / scale) + zero.  q (out, in), scale and zero (out, ceil(in / group)). */
+ * scale), q = round(w / scale) + zero, within 0..15.  A group that holds a NaN or an infinity is NaN throughout.  q (out, in), scale
+ * and zero (out, ceil(in / group)). */
 CARD_API int card_linear4_quantize(const float* W, int32_t out_features, int32_t in_features, int32_t group, uint8_t* q, float* scale,
                                    uint8_t* zero, void* stream);
 

@@ -81,3 +81,27 @@ def test_linear4_rows_near_the_end_of_the_range(dtype, rows, in_f, out_f):
     want, size = ref.linear4(q, s, z, b, 64, x)
     assert bool((want.abs() < 2.0 ** 127).all())
     assert_within(lin.forward(x, out_dtype=torch.float32), want, lin_bound(want, size, 64, in_f, torch.float32))
+
+
+def test_quantize_weight_of_odd_ranges():
+    """Ranges below the normal numbers and past the largest one; a group that holds a NaN or an infinity is NaN."""
+    group = 32
+    w = rand(9, 96, seed=3).clamp(-3, 3)
+    w[1] *= 2.0 ** -126
+    w[2] *= 2.0 ** -135
+    w[3] = w[3].abs() * 2.0 ** -130
+    w[4] = w[4].clamp(-1.9, 1.9) * 2.0 ** 127
+    w[4, 0], w[4, 1] = 1.9 * 2.0 ** 127, -1.9 * 2.0 ** 127
+    w[5, 40], w[6, 70], w[7, 3] = float("nan"), float("inf"), -float("inf")
+    q, s, z = card_amd.quantize_weight(w, group=group)
+    at = torch.arange(96) // group
+    step = s.cpu().double()[:, at]
+    deq = (q.cpu().double() - z.cpu().double()[:, at]) * step
+    w64 = w.cpu().double()
+    bad = torch.zeros(9, 96, dtype=torch.bool)
+    bad[5, 32:64], bad[6, 64:], bad[7, :32] = True, True, True
+    assert bool(torch.isnan(deq[bad]).all())
+    # a scale below the normal numbers is off by 2^-150, sixteen steps of it
+    bound = step * (0.5 + 20 * 4 * U32) + 4 * U32 * w64.abs() + 16 * 2.0 ** -150
+    assert bool(((deq - w64).abs() <= bound)[~bad].all())
+    assert bool((s[1:5] > 0).all()) and bool(torch.isfinite(s[:5]).all())
