@@ -1,6 +1,7 @@
 """ctypes binding of libcard_hip.so (include/card_hip.h).  Fails loudly if the library is missing."""
 import ctypes as C
 import os
+import weakref
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("CARD_AMD_LIB") or os.path.join(_HERE, "libcard_hip.so")  # override: kernel A/B builds
@@ -91,6 +92,18 @@ class Linear4Desc(C.Structure):
 
 class CardError(RuntimeError):
     pass
+
+
+class Handle(C.c_void_p):
+    """A library object and its life: `destroy` runs when the last holder of this handle is gone, so a shallow copy of a holder
+    keeps it.  There is no second one of the same object: deep copies and pickles are refused."""
+
+    def __init__(self, value, destroy):
+        super().__init__(value)
+        weakref.finalize(self, destroy, C.c_void_p(value))
+
+    def __reduce_ex__(self, protocol):
+        raise CardError("weights packed on a GPU are neither copied nor pickled; pack them again from the tensors or the module")
 
 
 _lib = None

@@ -53,8 +53,7 @@ class GuidanceNet:
         L = _lib.lib()
         with torch.cuda.device(device):
             _lib.check(L.card_fphi_create(C.byref(d), _stream(device), C.byref(h)), "card_fphi_create")
-        self._h = h
-        weakref.finalize(self, L.card_fphi_destroy, h)
+        self._h = _lib.Handle(h.value, L.card_fphi_destroy)
 
     @classmethod
     def from_module(cls, net, device=None, *, weight_bits=None, group=64):

@@ -10,7 +10,6 @@ contiguous are copied first, as everywhere in card_amd.
 """
 import ctypes as C
 import os
-import weakref
 
 import torch
 
@@ -69,7 +68,8 @@ def rms_norm_e4m3(x, weight=None, *, residual=None, eps=1e-6):
 
 class QuantLinear:
     """A Linear layer with 4-bit weights, packed on one GPU (on the current stream); immutable after construction
-    (card_linear4).  It holds the weights that a captured graph reads: keep it as long as the graph.
+    (card_linear4).  It holds the weights that a captured graph reads: keep it as long as the graph.  copy.copy shares them;
+    deep copies and pickles are refused.
 
     w[o, k] = (q[o, k] - zero[o, k // group]) * scale[o, k // group]: q (out, in) uint8 with values 0..15, scale (out,
     ceil(in / group)) float32, zero likewise uint8 (0..15) or None = 8 everywhere, bias (out,) or None; group 32, 64 or 128."""
@@ -103,8 +103,7 @@ class QuantLinear:
             _lib.check(L.card_linear4_create(C.byref(d), _stream(self.device), C.byref(h)), "card_linear4_create")
         self._index = self.device.index
         self.in_features, self.out_features, self.group = in_f, out_f, group
-        self._h = h.value
-        weakref.finalize(self, L.card_linear4_destroy, h)
+        self._h = _lib.Handle(h.value, L.card_linear4_destroy)
 
     @classmethod
     def from_float(cls, weight, bias=None, *, group=128, device=None):
@@ -117,7 +116,7 @@ class QuantLinear:
         x_scale (...,) float32, the scale of each row; gamma (out,) float32: a ConditionalLinear's embedding row; slope: a
         LeakyReLU's negative slope (0 = ReLU), None = no activation; out_dtype: x's type by default (bf16 for 8-bit rows).
         Made for one to some tens of rows, right for up to 65535."""
-        return (_ext or _load()).linear4(self._h, self._index, self.in_features, self.out_features, x, x_scale, gamma,
+        return (_ext or _load()).linear4(self._h.value, self._index, self.in_features, self.out_features, x, x_scale, gamma,
                                          1.0 if slope is None else slope, out_dtype)
 
     __call__ = forward

@@ -95,12 +95,10 @@ class Sampler:
             _lib.check(L.card_sampler_create(C.byref(d), _stream(device), C.byref(h)), "card_sampler_create")
             # the pack kernels read `keep` asynchronously on the current stream; the caching allocator is
             # stream-ordered, so releasing them after this point is safe
-        self._h = h
+        self._h = _lib.Handle(h.value, L.card_sampler_destroy)
         self.workspace_limit = None      # bytes; set to bound the GEMM back end's workspace (runs then go in chunks)
         self._ws = None                  # (tensor, aligned ptr, bytes): grown on demand, reused by later calls
         self._slot_cache = {}            # CARD_OUT_SELECT state -> slot tables on the device
-        self._destroy = L.card_sampler_destroy
-        weakref.finalize(self, L.card_sampler_destroy, h)
 
     # ------------------------------------------------------------------------------------------
     @classmethod

@@ -1,8 +1,14 @@
 """The layer operators at the edges of their range.  Tolerances count roundings, as in test_gpu_layers.py."""
+import copy
+import gc
+import pickle
+
 import pytest
 import torch
+from torch import nn
 
 import card_amd
+from card_amd._lib import CardError
 from tests import layer_reference as ref
 from tests.layer_reference import TINY, U, U32, assert_within
 from tests.test_gpu_layers import DEV, TYPES, chain, ids, lin_bound, rand, weights
@@ -105,3 +111,23 @@ def test_quantize_weight_of_odd_ranges():
     bound = step * (0.5 + 20 * 4 * U32) + 4 * U32 * w64.abs() + 16 * 2.0 ** -150
     assert bool(((deq - w64).abs() <= bound)[~bad].all())
     assert bool((s[1:5] > 0).all()) and bool(torch.isfinite(s[:5]).all())
+
+
+# ------------------------------------------------------------------------------------------------ copies
+def test_copies_of_packed_weights():
+    """A shallow copy holds the weights when the original is gone; other copies are refused."""
+    net = nn.Sequential(nn.Linear(96, 40), nn.LeakyReLU(), nn.Dropout(0.2), nn.Linear(40, 3)).to(DEV).eval()
+    x = rand(5, 96)
+    for make in (lambda: card_amd.QuantLinear(*weights(24, 96, 32, True), group=32), lambda: card_amd.GuidanceNet.from_module(net),
+                 lambda: card_amd.GuidanceNet.from_module(net, weight_bits=4)):
+        a = make()
+        want = a(x)
+        for how in (copy.deepcopy, pickle.dumps):
+            with pytest.raises(CardError, match="pack them again"):
+                how(a)
+        b = copy.copy(a)
+        del a
+        gc.collect()
+        others = [make() for _ in range(4)]          # would lie where freed weights were
+        assert torch.equal(b(x), want)
+        del others
