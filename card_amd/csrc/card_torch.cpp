@@ -5,6 +5,7 @@
 // Why not ctypes, as for the sampler: these calls take 3 to 20 us on the device, and a Python call with its checks, outputs
 // and launch took 7 to 12 us, one that goes through a Python autograd node 81 us forward and backward.
 #include <torch/extension.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -56,6 +57,13 @@ void same(const Tensor& t, const Tensor& like, at::IntArrayRef shape, const char
 Tensor dense(const OptTensor& t) { return t ? t->contiguous() : Tensor(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+// What would vanish without an error: a tangent (forward-mode derivative) of an input, and the kernels themselves in a trace, which
+// sees torch's calls only and would keep the outputs as they were allocated.
+template <typename... T> void check_mode(const char* what, const T&... inputs) {
+    if (at::tracer::impl::is_dispatch_enabled()) refuse(what, ": torch.jit.trace does not see the kernels; call it outside the trace");
+    const auto dual = [](const OptTensor& t) { return t && t->defined() && t->_fw_grad(0).defined(); };
+    if ((dual(inputs) || ...)) refuse(what, " has no forward-mode derivative");
+}
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool capturing(const c10::hip::HIPStream& s) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -64,7 +72,8 @@ bool capturing(const c10::hip::HIPStream& s) {
 // What a backward pass is refused for.  A leaf's gradient node remembers the stream it was made on, and lives as long as any
 // graph of the leaf.  Into a capture that began after it, the engine would draw that stream with a wait that is not allowed
 // there, and the process would not survive the capture's end.
-void check_backward(const char* what) {
+void check_backward(const char* what, const torch::autograd::tensor_list& grads) {
+    for (const Tensor& g : grads) check_mode(what, g);
     if (at::GradMode::is_enabled()) refuse(what, ": the backward pass is of first order only (create_graph=True asks for more)");
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
@@ -117,7 +126,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
         return drop_forward(x.contiguous(), dense(residual), dense(state), {(int)dtype, rows, cols, (int)n_z, p, (uint64_t)seed, (uint64_t)elem_offset, (int)draw});
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grads) {
-        check_backward("dropout");
+        check_backward("dropout", grads);
         const auto c = ctx->saved_data["call"].toIntVector();
         const auto saved = ctx->get_saved_variables();
         torch::autograd::tensor_list out(11);
@@ -134,6 +143,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 Tensor dropout(const Tensor& x, double p, uint64_t seed, const OptTensor& state_, int64_t elem_offset, int64_t draw, int64_t n_z, const OptTensor& residual) {
     on_gpu(x);
+    check_mode("dropout", x, residual);
     const int dtype = dtype_of(x, "dropout");
     if (x.dim() < 1) refuse("dropout: x is a scalar; expected (..., cols)");
     if (n_z < 1 || n_z > INT32_MAX || draw < 0 || draw > INT32_MAX || elem_offset < 0)
@@ -185,7 +195,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         return n.h.defined() ? torch::autograd::tensor_list{n.y, n.h} : torch::autograd::tensor_list{n.y};
     }
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grads) {
-        check_backward("rms_norm");
+        check_backward("rms_norm", grads);
         const auto saved = ctx->get_saved_variables();
         const Tensor h = saved[0], weight = saved[1];
         const Tensor g = grads[0].defined() ? grads[0].contiguous() : Tensor();
@@ -209,6 +219,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 // checks the arguments; whether a gradient is asked for
 bool norm_args(const char* what, const Tensor& x, const OptTensor& weight_, const OptTensor& residual) {
     on_gpu(x);
+    check_mode(what, x, weight_, residual);
     dtype_of(x, what);
     if (x.dim() < 1 || x.size(-1) < 1) refuse(what, ": x has shape ", x.sizes(), "; expected (..., cols) with cols >= 1");
     if (weight_) {
@@ -236,6 +247,7 @@ std::vector<Tensor> rms_norm_e4m3(const Tensor& x, const OptTensor& weight, cons
 Tensor linear4(uintptr_t handle, int64_t device, int64_t in, int64_t out, const Tensor& x, const OptTensor& x_scale_, const OptTensor& gamma_, double slope,
                const std::optional<at::ScalarType>& out_dtype) {
     on_gpu(x);
+    check_mode("QuantLinear", x, x_scale_, gamma_);
     const at::Device dev = x.device();
     if (dev.index() != device) refuse("QuantLinear: x is on ", dev.str(), ", the weights are on cuda:", device);
     if (x.dim() < 1 || x.size(-1) != in) refuse("QuantLinear: x has shape ", x.sizes(), "; expected (..., ", in, ")");

@@ -4,7 +4,8 @@ weights (card_linear4).
 
 All take fp32, bf16 and fp16 tensors on the GPU, launch on the current stream of the tensor's device, never synchronise and
 raise CardError for what the kernels do not cover.  `dropout` and `rms_norm` have a backward pass (of first order);
-a captured backward pass needs its forward pass in the same capture and no older graph of the same tensors.
+a captured backward pass needs its forward pass in the same capture and no older graph of the same tensors.  Tensors with a
+forward-mode tangent and calls under torch.jit.trace are refused.
 `rms_norm_e4m3` and `QuantLinear` are for inference and refuse tensors that ask for a gradient.  Tensors that are not
 contiguous are copied first, as everywhere in card_amd.
 """

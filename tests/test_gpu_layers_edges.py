@@ -131,3 +131,42 @@ def test_copies_of_packed_weights():
         others = [make() for _ in range(4)]          # would lie where freed weights were
         assert torch.equal(b(x), want)
         del others
+
+
+# ------------------------------------------------------------------------------------------------ derivatives
+def calls(x, w, lin):
+    return [lambda x: card_amd.dropout(x, 0.3, seed=1), lambda x: card_amd.dropout(x.detach(), 0.3, seed=1, residual=x), lambda x: card_amd.rms_norm(x, w),
+            lambda x: card_amd.rms_norm(x.detach(), w, residual=x)[0], lambda x: card_amd.rms_norm(x.detach(), x[0]), lambda x: card_amd.rms_norm_e4m3(x, w)[1],
+            lambda x: card_amd.rms_norm_e4m3(x.detach(), x[0])[1], lin, lambda x: lin(x.detach(), gamma=x[0, :8].contiguous())]
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+    x, t, w = rand(4, 64), rand(4, 64, seed=1), 1 + 0.1 * rand(64, seed=2)
+    lin = card_amd.QuantLinear(*weights(8, 64, 32, True), group=32)
+    for leaf in (False, True):
+        for k, call in enumerate(calls(x, w, lin)):
+            with fw.dual_level():
+                dual = fw.make_dual(x.clone().requires_grad_(leaf), t)
+                with pytest.raises(CardError, match="forward-mode|no backward"):
+                    call(dual)
+    a = x.clone().requires_grad_(True)
+    for y in (card_amd.dropout(a, 0.3, seed=1), card_amd.rms_norm(a, w)):
+        with fw.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, a, fw.make_dual(x, t), retain_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, a, torch.stack((x, t)), is_grads_batched=True)
+    for call in calls(x, w, lin):          # and behind the level all is as before
+        assert torch.isfinite(call(x)).all()
+
+
+def test_transforms_and_traces_are_refused():
+    x, w = rand(4, 64), 1 + 0.1 * rand(64, seed=2)
+    lin = card_amd.QuantLinear(*weights(8, 64, 32, True), group=32)
+    for call in calls(x, w, lin)[:1] + calls(x, w, lin)[2:3] + calls(x, w, lin)[5:6] + [lambda x: lin(x)]:          # a trace wants a function
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(x[None])
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (x,), (x,))
+        with pytest.raises(CardError, match="trace"):
+            torch.jit.trace(call, x, check_trace=False)
