@@ -223,7 +223,8 @@ def describe_guidance(net):
     LeakyReLU / ReLU / Dropout / RMSNorm / Identity -- and return {"dims": [dim_in, hidden..., dim_out], "weights": [Linear.weight
     ...], "biases": [...], "batchnorm": [the BatchNorm1d module that follows layer l, or None], "negative_slope": float,
     "dropout": [the Dropout rate behind hidden layer l] (None: Dropout layers elsewhere), "norms": [the RMSNorm ahead of layer l, or None]}
-    with the module's own Parameter objects.  Raises CardError for train-mode BatchNorm / Dropout and foreign layers."""
+    with the module's own Parameter objects.  Raises CardError for train-mode BatchNorm / Dropout, foreign layers and orders other
+    than Linear, [BatchNorm], activation -- which is what the kernels compute -- with Dropout anywhere."""
     import torch.nn as nn
     net = getattr(net, "module", net) if isinstance(net, (nn.DataParallel, nn.parallel.DistributedDataParallel)) else net
     seq = getattr(net, "network", net)
@@ -231,6 +232,8 @@ def describe_guidance(net):
     drops, norms, norm, active, simple = [], [], None, False, True
     for m in seq.children():
         if isinstance(m, nn.Linear):
+            if Ws and not active:
+                raise CardError("f_phi: a Linear layer behind another without an activation between them")
             Ws.append(m.weight)
             bs.append(m.bias)
             bns.append(None)
@@ -243,21 +246,19 @@ def describe_guidance(net):
             if m.training or not m.track_running_stats:
                 raise CardError("f_phi BatchNorm1d must be in eval mode with running statistics (the reference calls "
                                 "cond_pred_model.eval() before testing, regression/card_regression.py:951)")
-            if not Ws or bns[-1] is not None or norm is not None:
-                raise CardError("f_phi: BatchNorm1d must follow a Linear layer")
+            if not Ws or bns[-1] is not None or norm is not None or active:
+                raise CardError("f_phi: BatchNorm1d must follow a Linear layer, ahead of its activation")
             bns[-1] = m
             simple = simple and drops[-1] == 0
-        elif norm is not None and isinstance(m, (nn.LeakyReLU, nn.ReLU)):
-            raise CardError("f_phi: an activation between RMSNorm and its Linear layer")
-        elif isinstance(m, nn.LeakyReLU):
-            active = True
-            if slope is not None and slope != m.negative_slope:
-                raise CardError("f_phi: LeakyReLU layers with different slopes")
-            slope = m.negative_slope
-        elif isinstance(m, nn.ReLU):
-            if slope not in (None, 0.0):
-                raise CardError("f_phi: mixed activation slopes")
-            slope, active = 0.0, True
+        elif isinstance(m, (nn.LeakyReLU, nn.ReLU)):
+            s = m.negative_slope if isinstance(m, nn.LeakyReLU) else 0.0
+            if norm is not None:
+                raise CardError("f_phi: an activation between RMSNorm and its Linear layer")
+            if not Ws or (active and s != 0):          # a second ReLU changes nothing
+                raise CardError("f_phi: an activation stands once behind a Linear layer")
+            if slope is not None and slope != s:
+                raise CardError("f_phi: activations with different slopes")
+            slope, active = s, True
         elif isinstance(m, nn.Dropout):
             if m.training and m.p > 0:
                 raise CardError("f_phi Dropout must be in eval mode (identity); call .eval() on the guidance model")
@@ -278,6 +279,8 @@ def describe_guidance(net):
         raise CardError("f_phi: no Linear layer found")
     if norm is not None:
         raise CardError("f_phi: RMSNorm behind the output layer")
+    if active:
+        raise CardError("f_phi: an activation behind the output layer")
     simple = simple and drops[-1] == 0
     if bns[-1] is not None:
         raise CardError("f_phi: BatchNorm after the output layer is not part of regression/model.py:70-79")
