@@ -296,15 +296,21 @@ def describe_guidance(net):
 _gcache = weakref.WeakKeyDictionary()
 
 
+def _settings(net):
+    """What describe_guidance reads of a network besides its tensors: its modules in their order with the numbers they hold"""
+    names = ("training", "p", "negative_slope", "eps", "track_running_stats")
+    return tuple((type(m),) + tuple(getattr(m, n, None) for n in names) for m in net.modules())
+
+
 def guidance_for(f_phi):
     """The cached GuidanceNet of an `nn.Module` (DeterministicFeedForwardNeuralNetwork), or of an OLS coefficient tensor
     (1 + x_dim, y_dim); a GuidanceNet passes through.  Re-packed when the weights change (identity + content check, like
-    sampler_for)."""
+    sampler_for), or the modules' own numbers: Dropout rates, slopes, eps, train mode."""
     if isinstance(f_phi, GuidanceNet):
         return f_phi
     if torch.is_tensor(f_phi):
         return GuidanceNet.from_ols(f_phi)                 # a (1 + x_dim) x y_dim matrix: packing it is one tiny copy
-    fp = (_fingerprint(f_phi), bool(getattr(f_phi, "training", False)))
+    fp = (_fingerprint(f_phi), _settings(f_phi))
     hit = _gcache.get(f_phi)
     h = None
     if hit is not None and hit[0] == fp:
