@@ -11,7 +11,7 @@ import card_amd
 from card_amd._lib import CardError
 from tests import layer_reference as ref
 from tests.layer_reference import TINY, U, U32, assert_within
-from tests.test_gpu_layers import DEV, TYPES, chain, ids, lin_bound, rand, weights
+from tests.test_gpu_layers import DEV, TYPES, chain, ids, lin_bound, rand, rows8, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -170,3 +170,45 @@ def test_transforms_and_traces_are_refused():
             torch.func.jvp(call, (x,), (x,))
         with pytest.raises(CardError, match="trace"):
             torch.jit.trace(call, x, check_trace=False)
+
+
+@pytest.mark.parametrize("rows,in_f,out_f", [(128, 200, 72), (512, 1000, 130), (6400, 136, 48), (65535, 100, 40), (1000, 70, 4200), (300, 40, 16400)])
+@pytest.mark.parametrize("dtype", TYPES + [torch.float8_e4m3fn], ids=ids)
+def test_linear4_of_many_rows(dtype, rows, in_f, out_f):
+    q, s, z, b = weights(out_f, in_f, 64, True)
+    lin = card_amd.QuantLinear(q, s, z, b, group=64)
+    x, xs = rows8(rows, in_f) if dtype is torch.float8_e4m3fn else (rand(rows, in_f, seed=5, dtype=dtype), None)
+    want, size = ref.linear4(q, s, z, b, 64, x, xs, None, 0.01)
+    y = lin.forward(x, xs, slope=0.01)
+    assert_within(y, want, lin_bound(want, size, 64, in_f, y.dtype))
+    # a row is the same in a call of few rows of the same form (more than 16)
+    part = slice(rows - 20, rows)
+    assert torch.equal(lin.forward(x[part], None if xs is None else xs[part], slope=0.01), y[part])
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantize_weight_is_the_nearest(group):
+    """q = round(w / scale) + zero clamped to 0..15: off by half a step at most, also at the ends of the range, where what the
+    clamp takes away is what rounding the zero point moved."""
+    w = rand(61, 333, seed=3) + 0.5 * rand(61, 1, seed=4)
+    q, s, z = card_amd.quantize_weight(w, group=group)
+    at = torch.arange(333) // group
+    step = s.cpu().double()[:, at]
+    deq = (q.cpu().double() - z.cpu().double()[:, at]) * step
+    w64 = w.cpu().double()
+    # scale, its reciprocal and the quotient are rounded: a few 2^-24 of |w| + 15 steps
+    assert bool(((deq - w64).abs() <= step * (0.5 + 20 * 4 * U32) + 4 * U32 * w64.abs()).all())
+
+
+@pytest.mark.parametrize("rows,in_f,out_f,group", [(13, 465, 13, 128), (1, 4096, 512, 128), (60, 70, 9, 64), (24, 4096, 5000, 32), (20, 2048, 16400, 64), (16, 12000, 100, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float8_e4m3fn], ids=ids)
+def test_linear4_fp32_results_of_short_rows(dtype, rows, in_f, out_f, group):
+    """fp32 results of rows of 8 and 16 bits are as exact as a product of 32 bits, root mean square: products of bf16 and e4m3 rows
+    have 13 bits at most, and their sums over a group are all but exact; those of fp16 rows have 16, and the two sums, some five
+    times their difference together, are rounded at their last place."""
+    q, s, z, b = weights(out_f, in_f, group, True)
+    x, xs = rows8(rows, in_f) if dtype is torch.float8_e4m3fn else (rand(rows, in_f, seed=5, dtype=dtype), None)
+    want, _ = ref.linear4(q, s, z, None, group, x, xs)
+    y = card_amd.QuantLinear(q, s, z, group=group)(x, xs, out_dtype=torch.float32).cpu().double()
+    n = -(-in_f // 32) + -(-in_f // group)
+    assert float((y - want).norm() / want.norm()) <= (n ** 0.5 + (5 if dtype is torch.float16 else 0)) * U32
