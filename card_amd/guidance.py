@@ -299,7 +299,8 @@ _gcache = weakref.WeakKeyDictionary()
 def _settings(net):
     """What describe_guidance reads of a network besides its tensors: its modules in their order with the numbers they hold"""
     names = ("training", "p", "negative_slope", "eps", "track_running_stats")
-    return tuple((type(m),) + tuple(getattr(m, n, None) for n in names) for m in net.modules())
+    numbers = lambda m: (v if isinstance(v, (int, float)) else None for v in (getattr(m, n, None) for n in names))  # noqa: E731
+    return tuple((type(m), *numbers(m)) for m in net.modules())
 
 
 def guidance_for(f_phi):

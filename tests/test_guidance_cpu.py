@@ -4,7 +4,7 @@ import torch
 from torch import nn
 
 from card_amd._lib import CardError
-from card_amd.guidance import _bn_fold, describe_guidance
+from card_amd.guidance import _bn_fold, _settings, describe_guidance
 
 
 def evaluate(d, x):
@@ -74,3 +74,13 @@ def test_a_description_computes_its_module(name):
 def test_orders_that_the_networks_do_not_compute_are_refused(name):
     with pytest.raises(CardError, match="f_phi"):
         describe_guidance(nn.Sequential(*REFUSED[name]()).eval())
+
+
+def test_settings_are_numbers():
+    """A module of another kind around the network may hold anything under these names."""
+    net = nn.Sequential(*ACCEPTED["the reference's order"]()).eval()
+    net.eps, net.p = torch.ones(3), nn.Linear(2, 2)
+    assert _settings(net) == _settings(net)
+    before = _settings(net)
+    net[3].p = 0.3
+    assert _settings(net) != before
