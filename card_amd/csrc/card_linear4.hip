@@ -3,7 +3,8 @@
 //   y[m, o] = act(gamma[o] * (x_scale[m] * sum_k (q[o, k] - zero[o, k / group]) * scale[o, k / group] * x[m, k] + bias[o]))
 //   act(v) = v > 0 ? v : slope * v
 //
-// The differences q - zero are small integers, exact in every type; products and sums are fp32, y is rounded once.
+// The differences q - zero are small integers, exact in every type; products and sums are fp32, y is rounded once.  Sums that are
+// not finite on the way are formed again from these differences (plain_sum).
 #include <new>
 
 #include "card_layers.h"
@@ -243,7 +244,9 @@ template <int G, int NT, bool STREAM> struct Weights {
 // fp32 rows: P and S are some five times their difference, and sums over a group lose that much at their last bit.  So the
 // first part's P and S, products of 13 bits, are taken for 32 columns each, where next to nothing is rounded; only the smaller
 // parts' run over the group.  Off by (root mean square) 6.7e-8 instead of 5.6e-7 at 465 columns, 1.1e-7 and 9.1e-7 at 4096, a
-// plain fp32 product 1.9e-7 and 5.8e-7; it costs 16 rows of 8192 x 28672 52.6 us for 44.5, of 4096 x 4096 8.9 for 8.3.
+// plain fp32 product 1.9e-7 and 5.8e-7; it costs 16 rows of 8192 x 28672 52.6 us for 44.5, of 4096 x 4096 8.9 for 8.3.  Shorter
+// rows are as exact without: bf16 and e4m3 products have 13 bits at most (fp32 results off by 4e-8 to 1.1e-7 at 70 to 12000
+// columns), fp16's 16 (1.2e-7 to 1.9e-7).
 template <int X, int G, int MT, int NT, bool STREAM, typename F>
 __device__ __forceinline__ void add_block(const Weights<G, NT, STREAM>& w, uint32_t sixteen, f32x4 (&acc)[MT][NT], F part) {
     constexpr int P = Row8<X>::kParts, S = 4 / G;          // S steps of 32 columns in a group
@@ -511,10 +514,12 @@ int splits_of(int tiles, int blocks, int64_t rows, int x_dtype) {
 // Several tiles share the values of x where there are more tiles than CUs (24 rows, 6144 outputs: 9.8 us with two against
 // 10.3).  From 1024 tiles on the weights pass by the caches, which cannot hold them (16 rows of 8192 columns, 28672 outputs:
 // 29.7 us against 31.5; but 5.8 against 5.1 for 4096 x 4096, whose weights stay in L2 from call to call), and workgroups are
-// plenty: four tiles and four waves with one block on its way, so that a CU holds four workgroups (8192 columns, 28672
-// outputs: 16 rows bf16 30.2 us against 34.8 with two tiles, eight waves and two blocks, 32 rows e4m3 40.0 and 51.1).  Up to
-// 16 rows of e4m3, half of bf16's x to read, need only three tiles to share them, and smaller workgroups even out the last ones
-// (28672 outputs 29.4 us against 29.9 with four, 17000 outputs of 4096 columns 12.2 and 14.5; but bf16 33.0 against 30.2).
+// plenty: four tiles and four waves with one block on its way, workgroups small enough that a CU holds several: up to 16 rows
+// three or two in 16 bits (152 to 175 registers), four to two in e4m3, two in fp32; 17 rows and more two, but one in e4m3 with
+// groups of 64 (263 registers).  8192 columns, 28672 outputs: 16 rows bf16 30.2 us against 34.8 with two tiles, eight waves and
+// two blocks, 32 rows e4m3 40.0 and 51.1.  Up to 16 rows of e4m3, half of bf16's x to read, need only three tiles to share them,
+// and smaller workgroups even out the last ones (28672 outputs 29.4 us against 29.9 with four, 17000 outputs of 4096 columns 12.2
+// and 14.5; but bf16 33.0 against 30.2).  All of these were measured with groups of 128.
 constexpr int kCus = 256, kStreamTiles = 1024;
 template <int X, int G, int MT> int by_tiles(const Args& a, const void* x, void* y, hipStream_t st) {
     // blocks on their way: one where rows are wide -- more than 16, or fp32 with its three operands -- for the registers' sake

@@ -10,7 +10,9 @@
 //
 // What bounds it is memory: a row is read once and lives in registers, V vectors of 16 bytes in each thread of a workgroup
 // of as many waves as the row needs (up to 64 vectors: 8, 16, 32 or 64 lanes).  A workgroup walks over rows with the weight in
-// registers and asks for the next row before it joins the sums of this one, so loads are on their way all the time.
+// registers and asks for the next row before it joins the sums of this one, so loads are on their way all the time.  Long
+// rows do not fit wholly: forward spills 14 to 87 registers to scratch where rows pass 64 KB (fp32 without e4m3: 128 KB), backward
+// 18 for 8193 to 16384 columns in 16 bits.
 // 8192 x 6144 bf16 with residual: forward 60 us (6.7 TB/s), backward 68 us (6.0 TB/s) and 4 us to join dw; 8192 x 4096 to e4m3
 // 44 us back to back (5.3 TB/s); one row of 4096 2.5 us.  A large copy reaches 5.5 TB/s on this card.
 #include "card_layers.h"
@@ -235,7 +237,8 @@ __global__ __launch_bounds__(L ? kThreads : 1024) void rms_norm_kernel(const Nor
     }
 }
 
-// Six waves to a SIMD (80 registers) are worth more than the last registers: 40000 x 1000 bf16 71 us against 89.
+// Six waves to a SIMD (80 registers) are worth more than the last registers: 40000 x 1000 bf16 71 us against 89.  The 64-bit form
+// (90 registers in fp32, 120 in 16 bits) and the one of two vectors a thread (106 and 128) run five and four.
 // F: in rows of a few columns the two terms of dx all but cancel (at one column to eps * rstd^2 of either), so there the
 // row's numbers and the difference are formed in 64 bits.
 template <typename T, typename F, int L, int V, bool STREAM>
@@ -415,7 +418,9 @@ __global__ __launch_bounds__(kJoinThreads) void dw_join_kernel(const float* part
 
 constexpr int kMaxCols = CARD_NORM_MAX_COLS;
 constexpr int kCus = 256;
-constexpr int kForwardWaves = 32, kBackwardWaves = 24;          // that a CU holds at a time: what the registers allow
+// Waves to a CU that workgroups are launched for: what the forms of one vector a thread have registers for.  With more vectors and
+// in the 64-bit form a CU holds 16 to 20, and the workgroups past those start when the first ones end.
+constexpr int kForwardWaves = 32, kBackwardWaves = 24;
 
 struct Form { int lanes, v, threads; };    // lanes per row (0: a workgroup of `threads`), vectors per thread
 Form form_of(int64_t cols, int n) {
@@ -427,7 +432,7 @@ Form form_of(int64_t cols, int n) {
     const int waves = (vecs + 64 * v - 1) / (64 * v);
     return {0, v, 64 * waves};
 }
-// workgroups that walk over the rows: as many as the chip holds at a time
+// workgroups that walk over the rows
 long long groups(const Form& f, int64_t rows, int waves) {
     const long long rpw = f.lanes ? kThreads / f.lanes : 1, g = (rows + rpw - 1) / rpw, per_cu = waves / (f.threads / 64);
     const long long most = kCus * (per_cu > 0 ? per_cu : 1);
